@@ -203,6 +203,60 @@ int tvllm_paged_decode_noalloc(const void* q, int64_t q_token_stride,
                                int dtype, int cache_dtype, float k_scale,
                                float v_scale, tvllm_stream_t stream);
 
+/* Decode attention for a batch whose rows share long prefixes, each computed
+ * once for its group of rows. No counterpart in the reference (its decode
+ * kernel reads a shared page once per row).
+ *
+ * A plan cuts one call's work into tasks. tvllm_shared_prefix_plan runs on the
+ * host (no GPU call) and fills `plan`, a host buffer of at least
+ * tvllm_shared_prefix_plan_words int32 words, which the caller copies to the
+ * device; one plan serves every layer of a step.
+ *   lengths[r] is row r's context (0: padding, its output is zeros);
+ *   groups[r] its group, or -1; the first prefix_lens[g] tokens (whole blocks)
+ *   of every row of group g lie in the same blocks, the rows' tables naming
+ *   them alike. lengths[r] >= prefix_lens[groups[r]]. A group of one row
+ *   shares nothing. All host pointers.
+ * num_tasks receives the number of tasks (the grid; at most
+ * tvllm_shared_prefix_max_tasks), workspace_bytes what the call needs (at most
+ * tvllm_shared_prefix_workspace_size). A plan buffer whose contents change
+ * between the replays of a captured call takes those two bounds as the call's
+ * num_tasks and workspace_bytes, and plans of the captured number of rows.
+ * 0 from the three sizes: invalid geometry (heads not divisible by KV heads,
+ * more than 2^20 rows, 4096 heads or 2^26 of both). */
+int64_t tvllm_shared_prefix_plan_words(int64_t max_rows, int64_t num_heads,
+                                       int64_t num_kv_heads);
+int64_t tvllm_shared_prefix_max_tasks(int64_t max_rows, int64_t num_heads,
+                                      int64_t num_kv_heads);
+int64_t tvllm_shared_prefix_workspace_size(int64_t max_rows, int64_t num_heads,
+                                           int64_t num_kv_heads, int64_t head_dim);
+int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* groups,
+                             const int64_t* prefix_lens, int64_t num_rows,
+                             int64_t num_groups, int64_t max_rows, int64_t num_heads,
+                             int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                             int32_t* plan, int64_t plan_words, int64_t* num_tasks,
+                             int64_t* workspace_bytes);
+
+/* tvllm_paged_decode's function by such a plan (on the device; max_rows, the
+ * geometry and block_size are those it was made with, or nothing is written):
+ * q, out, caches, rows, blocks and offsets as there; the context lengths are
+ * the plan's. head_dim a multiple of 8 up to 256; cache rows in aligned
+ * 8-element units, q rows 16-byte aligned, out rows 8-byte. workspace (16-byte
+ * aligned, no initialisation) holds the partial results of this call; calls
+ * that may overlap need their own. fp32 softmax and sums; the weights enter
+ * the products as two 16-bit terms of the cache's type, or, over keys shared by
+ * more than 16 query vectors of a KV head, as fp16 (11 bits; 2^-32 of the
+ * row's largest where that is more). An infinity or NaN in V makes the outputs
+ * that attend it non-finite. */
+int tvllm_paged_decode_shared_prefix(
+    const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+    const void* v_cache, void* out, int64_t out_token_stride, int64_t out_head_stride,
+    const int64_t* rows, const int64_t* blocks, const int64_t* offsets, const int32_t* plan,
+    int64_t num_rows, int64_t max_rows, int64_t num_tasks, int64_t num_heads,
+    int64_t num_kv_heads, int64_t head_dim, int64_t num_slots, int64_t cache_slot_stride,
+    int64_t cache_head_stride, int64_t block_size, float scale, void* workspace,
+    int64_t workspace_bytes, int dtype, int cache_dtype, float k_scale, float v_scale,
+    tvllm_stream_t stream);
+
 /* tvllm_qk_norm_rope's fused KV write followed by tvllm_paged_decode, in
  * one kernel, for a step whose rows are all decode rows: q, k, v are the raw
  * projections (element strides, last 1); each workgroup normalises and

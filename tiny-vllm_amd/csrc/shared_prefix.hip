@@ -1,0 +1,1072 @@
+// Decode attention for batches whose rows share a long prefix, computed once
+// for all of them.
+//
+// For decode row r and query head h,
+//   out[rows[r], h] = sum_t softmax_t(scale * q . k_t) v_t,  t < lengths[r],
+// exactly as paged decode, but the first prefix_lens[g] tokens of the rows of
+// group g lie in the same pages. The softmax splits over any partition X of
+// the keys: with m_X = max s, l_X = sum e^(s - m_X), a_X = sum e^(s - m_X) v,
+//   out = sum_X e^(m_X - m) a_X / sum_X e^(m_X - m) l_X,  m = max_X m_X,
+// so a group's shared keys are one part that every query of the group takes
+// from one read of K and V, and each row's own keys are others.
+//
+// The reference has no counterpart (its decode reads a shared page once per
+// row: tinyvllm/kernels/paged_decode.cu:92-466).
+//
+// MI355X design:
+//  * A host-side planner cuts the work into tasks - (KV head, range of keys,
+//    up to 128 query vectors) for shared keys, (row, KV head, range of keys)
+//    for own ones - of about equal length, 512 of them (two workgroups on each
+//    of 256 CUs) where the keys allow. One launch runs them all, so the
+//    compute-bound shared part and the memory-bound own parts overlap; a
+//    second merges the parts of each (row, head).
+//  * Wide tasks (above 16 query vectors): K/V tiles of 64 tokens in LDS, 32
+//    queries per wave on the 32x32x16 MFMA: S^T = K Q^T leaves a lane with 16
+//    tokens of its own query, which are the k values of its column in O^T +=
+//    V^T P^T, so P never moves. V is read from LDS through the transposing
+//    load, so it is staged as it lies in the cache.
+//  * Narrow tasks (up to 16 query vectors; a row's own keys at GQA groups up
+//    to 16): each of four waves streams its quarter of the keys straight into
+//    registers, Q.K^T and P.V on 16-wide MFMAs, and the waves merge in LDS.
+#include "common.h"
+
+#include <algorithm>
+#include <type_traits>
+#include <vector>
+
+namespace tvllm {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kThreads = 256;
+constexpr int kWide = 128;    // query vectors of a wide task (32 per wave)
+constexpr int kNarrow = 16;   // query vectors of a narrow one
+constexpr float kLog2e = 1.4426950408889634f;
+// Running maxima of the wide path rise only when a tile's maximum exceeds them
+// by more than this (log2 units), so most tiles skip the rescale.
+constexpr float kSlack = 8.f;
+// P enters the products as fp16: weights are carried at 2^kShift times their
+// value, so that with the slack they stay below 2^15 and keep all 11 bits down
+// to 2^-21 of the running maximum, a part of 2^-32 of it below.
+constexpr float kShift = 7.f;
+
+// ------------------------------------------------------------------ plan --
+// int32 words: header | per row (first part, parts) | members | tasks.
+constexpr int kHeader = 16;
+constexpr int kTaskWords = 8;
+enum Header { H_TASKS, H_ROWS, H_HEADS, H_KV_HEADS, H_DIM, H_BLOCK, H_PARTS };
+// A task's queries are number q_begin .. + q_count - 1 of its group's, query i
+// being head i % group (of the KV head) of row members[member + i / group]; its
+// keys are tokens k0 .. k1 - 1 of the first such row's table.
+enum Task { T_MEMBER, T_QBEGIN, T_QCOUNT, T_KVH, T_K0, T_K1, T_PART, T_UNUSED };
+
+constexpr int64_t kTargetTasks = 512;  // two workgroups per CU
+constexpr int64_t kKeyUnit = 64;       // tasks' key ranges are multiples of this
+constexpr int64_t kMinKeys = 256;      // no split makes shorter tasks
+constexpr int64_t kMaxParts = 64;      // splits of one unit
+
+struct PlanLayout {
+    int64_t rows_at, members_at, tasks_at, max_tasks, words;
+};
+
+PlanLayout plan_layout(int64_t max_rows, int64_t heads, int64_t kv_heads) {
+    const int64_t group = heads / kv_heads;
+    PlanLayout p;
+    // Every unit (KV head, tile of queries) of keys K makes at most K / chunk
+    // + 1 tasks, and chunk >= all units' keys / kTargetTasks.
+    const int64_t own = max_rows * ((group + kWide - 1) / kWide);
+    const int64_t shared = (max_rows * group + kWide - 1) / kWide + max_rows / 2;
+    p.max_tasks = kTargetTasks + kv_heads * (own + shared);
+    p.rows_at = kHeader;
+    p.members_at = p.rows_at + 2 * max_rows;
+    p.tasks_at = p.members_at + max_rows;
+    p.words = p.tasks_at + kTaskWords * p.max_tasks;
+    return p;
+}
+
+// (row part, query head) results of one call at most: a unit of q queries and
+// K keys makes q (K / chunk + 1) of them.
+int64_t max_entries(int64_t max_rows, int64_t heads) {
+    return 2 * max_rows * heads + kWide * kTargetTasks;
+}
+
+// ---------------------------------------------------------------- device --
+
+template <typename T>
+struct Args {
+    const T* q;
+    int64_t qts, qhs;
+    const void* k;  // cache rows: T elements, or FP8 E4M3 bytes
+    const void* v;
+    int64_t css, chs;  // cache slot / head strides (elements)
+    T* out;
+    int64_t ots, ohs;
+    const int64_t* rows;
+    const int64_t* blocks;
+    const int64_t* offsets;
+    const int32_t* plan;
+    int rows_at, members_at, tasks_at;
+    int num_rows, heads, kv_heads, group, head_dim, block_size;
+    uint32_t page_mul;  // t / block_size == (t * page_mul) >> page_shift, t < 2^31
+    int page_shift;
+    float scale_log2;  // softmax scale * log2(e) (* k_scale for an FP8 cache)
+    float v_scale;     // FP8 cache: V dequantisation scale (1 otherwise)
+    float* part_o;     // [entries][head_dim], unnormalised
+    float2* part_ml;   // [entries]: (max, sum) in base 2
+    int64_t entries;   // room in the two
+};
+
+__device__ __forceinline__ float as_f(uint32_t x) { return __uint_as_float(x); }
+__device__ __forceinline__ uint32_t as_u(float x) { return __float_as_uint(x); }
+
+// D[32x32] += A[32x16] B[16x32]. Lane l: A row l%32 and B column l%32 with
+// k = 8*(l/32)..+7; D column l%32, rows 8*(v/4) + 4*(l/32) + v%4 for v < 16.
+template <typename T>
+__device__ __forceinline__ f32x16 mfma_32x32x16(const U16x8& a, const U16x8& b, f32x16 c) {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    if constexpr (std::is_same_v<T, __bf16>) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(t8, a),
+                                                       __builtin_bit_cast(t8, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(t8, a),
+                                                      __builtin_bit_cast(t8, b), c, 0, 0, 0);
+    }
+}
+
+// D[16x16] += A[16x16] B[16x16]: lane l supplies A row l%16 and B column l%16
+// with k = 4*(l/16)..+3; D column l%16, rows 4*(l/16) + v.
+template <typename T>
+__device__ __forceinline__ f32x4 mfma_16x16x16(uint2 a, uint2 b, f32x4 c) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    if constexpr (std::is_same_v<T, __bf16>) {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
+            __builtin_bit_cast(s4, a), __builtin_bit_cast(s4, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(
+            __builtin_bit_cast(h4, a), __builtin_bit_cast(h4, b), c, 0, 0, 0);
+    }
+}
+
+// Transposing LDS read: lanes 16b + 4r + c of each 16-lane block b point at 4
+// consecutive 16-bit elements, row r, columns 4c..4c+3 of a 4 x 16 block; lane
+// 16b + x gets column x, rows 0..3.
+__device__ __forceinline__ uint2 read_transposed(const uint16_t* p) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    return __builtin_bit_cast(
+        uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                   (lds_s4*)(const __attribute__((address_space(3))) uint16_t*)p));
+}
+
+// Lanes l and l + 32 hold the same query: combine them with one row swap.
+__device__ __forceinline__ float pair_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(as_u(x), as_u(x), false, false);
+    return fmaxf(as_f(r[0]), as_f(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(as_u(x), as_u(x), false, false);
+    return as_f(r[0]) + as_f(r[1]);
+}
+
+// N bytes from memory as they lie there; rows read once go past the caches.
+template <int N>
+struct Bytes {
+    uint32_t w[(N + 3) / 4];
+};
+
+template <int N>
+__device__ __forceinline__ Bytes<N> load_bytes(const char* p) {
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    Bytes<N> r;
+    if constexpr (N == 2) {
+        r.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(p));
+    } else if constexpr (N == 4) {
+        r.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+    } else if constexpr (N == 8) {
+        const u2 t = __builtin_nontemporal_load(reinterpret_cast<const u2*>(p));
+        r.w[0] = t[0];
+        r.w[1] = t[1];
+    } else {
+        static_assert(N == 16);
+        const u4 t = __builtin_nontemporal_load(reinterpret_cast<const u4*>(p));
+        r.w[0] = t[0];
+        r.w[1] = t[1];
+        r.w[2] = t[2];
+        r.w[3] = t[3];
+    }
+    return r;
+}
+
+// Two E4M3 bytes (the low or high half of w) -> two T elements, exact.
+template <typename T, bool HI>
+__device__ __forceinline__ uint32_t widen2(uint32_t w) {
+    if constexpr (std::is_same_v<T, __bf16>) {
+        return __builtin_bit_cast(uint32_t,
+                                  __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI));
+    } else {
+        return __builtin_bit_cast(uint32_t,
+                                  __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI));
+    }
+}
+
+template <typename T, int DP, bool F8>
+__global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2)
+shared_prefix_tasks(Args<T> a) {
+    constexpr int EB = F8 ? 1 : 2;             // bytes per cached element
+    constexpr int BK = DP == 256 ? 32 : 64;    // tokens per wide tile
+    constexpr int K_LD = DP + 8;               // LDS row strides (elements): 16-byte reads
+    constexpr int V_LD = DP == 32 ? 32 : DP + 32;  // and transposing reads without conflicts
+    constexpr int K_TILE = BK * K_LD, V_TILE = BK * V_LD;
+    constexpr int kTileBytes = 2 * 2 * (K_TILE + V_TILE);
+    constexpr int kMergeBytes = 4 * kNarrow * (4 * DP + 8);
+    __shared__ __align__(16) char lds[kTileBytes > kMergeBytes ? kTileBytes : kMergeBytes];
+
+    const int32_t* const plan = a.plan;
+    if (int(blockIdx.x) >= plan[H_TASKS] || plan[H_ROWS] != a.num_rows ||
+        plan[H_HEADS] != a.heads || plan[H_KV_HEADS] != a.kv_heads ||
+        plan[H_DIM] != a.head_dim || plan[H_BLOCK] != a.block_size ||
+        plan[H_PARTS] > a.entries)
+        return;
+    const int32_t* const task = plan + a.tasks_at + int64_t(blockIdx.x) * kTaskWords;
+    const int32_t* const members = plan + a.members_at + task[T_MEMBER];
+    const int q_begin = task[T_QBEGIN], q_count = task[T_QCOUNT], kvh = task[T_KVH];
+    const int k0 = task[T_K0], k1 = task[T_K1], part = task[T_PART];
+    const int D = a.head_dim;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int64_t table = a.offsets[members[q_begin / a.group]];
+    const uint32_t* const ids = reinterpret_cast<const uint32_t*>(a.blocks + table);
+    const uint32_t row_bytes = uint32_t(a.css * EB);
+    const char* const kbase = static_cast<const char*>(a.k) + int64_t(kvh) * a.chs * EB;
+    const char* const vbase = static_cast<const char*>(a.v) + int64_t(kvh) * a.chs * EB;
+
+    auto page_of = [&](uint32_t t) {
+        return uint32_t((uint64_t(t) * a.page_mul) >> a.page_shift);
+    };
+    auto slot_of = [&](uint32_t id, uint32_t t, uint32_t page) {
+        return id * uint32_t(a.block_size) + (t - page * uint32_t(a.block_size));
+    };
+    // Query i of the task: its row, and its head.
+    auto query = [&](int i, int& row, int& head) {
+        const int g = (q_begin + i) / a.group;
+        row = members[g];
+        head = kvh * a.group + (q_begin + i - g * a.group);
+    };
+    // Where a row's part goes; rows of one part are written to the output.
+    auto entry_of = [&](int row, int head, bool& direct) -> int64_t {
+        const int first = plan[a.rows_at + 2 * row];
+        direct = plan[a.rows_at + 2 * row + 1] == 1;
+        return (int64_t(first) + part) * a.heads + head;
+    };
+
+    // ------------------------------------------------------------- wide --
+    // Returns whether the outputs are not what fp16 V can give (see below).
+    auto wide = [&]() -> bool {
+        constexpr int PPR = DP / 8;               // 8-element pieces per row
+        constexpr int JP = BK * PPR / kThreads;   // pieces per thread, K and V each
+        constexpr int TB = BK / 32;
+        constexpr int NC = DP / 16, ND = DP / 32;
+        constexpr int EBP = 8 * EB;
+        // A bf16 cache's V enters the products as fp16 (P needs its 11 bits: a
+        // bf16 P is 2^-9 off, as much as the output's own rounding). That is
+        // exact below 65536 in magnitude, to 2^-25 below 2^-14; beyond, the
+        // outputs it reaches end non-finite and the task is done again by the
+        // narrow path, which takes V as it is.
+        constexpr bool kConvert = std::is_same_v<T, __bf16> && !F8;
+        uint16_t* const ks = reinterpret_cast<uint16_t*>(lds);
+        uint16_t* const vs = ks + 2 * K_TILE;
+        const int col = lane & 31, half = lane >> 5;
+        const int qi = wave * 32 + col;
+        const bool active = wave * 32 < q_count;
+        int row, head;
+        query(min(qi, q_count - 1), row, head);
+
+        U16x8 qv[NC];
+        {
+            const T* qrow = a.q + a.rows[row] * a.qts + head * a.qhs;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int d = 16 * c + 8 * half;
+                qv[c] = d < D ? *reinterpret_cast<const U16x8*>(qrow + d) : U16x8{};
+            }
+        }
+
+        const int ntiles = (k1 - k0 + BK - 1) / BK;
+        const uint32_t last = uint32_t(k1 - 1);
+        uint32_t id[JP];
+        Bytes<EBP> kst[JP], vst[JP];
+        auto token_of = [&](int i, int j) {  // past the end: the last token again
+            return min(uint32_t(k0 + i * BK + (tid + j * kThreads) / PPR), last);
+        };
+        auto load_ids = [&](int i) {
+#pragma unroll
+            for (int j = 0; j < JP; ++j) id[j] = ids[2 * uint64_t(page_of(token_of(i, j)))];
+        };
+        auto load_tile = [&](int i) {
+#pragma unroll
+            for (int j = 0; j < JP; ++j) {
+                const uint32_t t = token_of(i, j);
+                const int piece = (tid + j * kThreads) % PPR;
+                const uint64_t off = uint64_t(slot_of(id[j], t, page_of(t))) * row_bytes +
+                                     uint32_t((piece * 8 < D ? piece : 0) * EBP);
+                kst[j] = load_bytes<EBP>(kbase + off);
+                vst[j] = load_bytes<EBP>(vbase + off);
+            }
+        };
+        auto store_tile = [&](int i) {
+            uint16_t* const kt = ks + (i & 1) * K_TILE;
+            uint16_t* const vt = vs + (i & 1) * V_TILE;
+            const int left = k1 - k0 - i * BK;
+#pragma unroll
+            for (int j = 0; j < JP; ++j) {
+                const int tok = (tid + j * kThreads) / PPR;
+                const int piece = (tid + j * kThreads) % PPR;
+                // Rows past the end and dims past the head's are zeros.
+                const bool keep = tok < left && piece * 8 < D;
+                U16x8 kw, vw;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    if constexpr (F8) {
+                        kw.w[w] = (w & 1) ? widen2<T, true>(kst[j].w[w >> 1])
+                                          : widen2<T, false>(kst[j].w[w >> 1]);
+                        vw.w[w] = (w & 1) ? widen2<_Float16, true>(vst[j].w[w >> 1])
+                                          : widen2<_Float16, false>(vst[j].w[w >> 1]);
+                    } else {
+                        kw.w[w] = kst[j].w[w];
+                        vw.w[w] = kConvert ? pack2<_Float16>(half_lo<T>(vst[j].w[w]),
+                                                             half_hi<T>(vst[j].w[w]))
+                                           : vst[j].w[w];
+                    }
+                    kw.w[w] = keep ? kw.w[w] : 0u;
+                    vw.w[w] = keep ? vw.w[w] : 0u;
+                }
+                *reinterpret_cast<U16x8*>(kt + tok * K_LD + piece * 8) = kw;
+                *reinterpret_cast<U16x8*>(vt + tok * V_LD + piece * 8) = vw;
+            }
+        };
+
+        f32x16 o[ND];  // O^T: lane = (dims 32n + 8g + 4*half + i, query col)
+#pragma unroll
+        for (int n = 0; n < ND; ++n) o[n] = f32x16{};
+        float m_run = -INFINITY, l_run = 0.f;
+
+        load_ids(0);
+        load_tile(0);
+        load_ids(1);
+        store_tile(0);
+        load_tile(1);
+        load_ids(2);
+        for (int i = 0; i < ntiles; ++i) {
+            // Tile i is in LDS, and nobody reads tile i - 1 any more.
+            __syncthreads();
+            store_tile(i + 1);
+            load_tile(i + 2);
+            load_ids(i + 3);
+            if (!active) continue;
+            const uint16_t* const kt = ks + (i & 1) * K_TILE;
+            const uint16_t* const vt = vs + (i & 1) * V_TILE;
+
+            f32x16 sc[TB];  // S^T: token 32tb + 8(v/4) + 4*half + v%4
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb) sc[tb] = f32x16{};
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int tb = 0; tb < TB; ++tb) {
+                    const U16x8 kk = *reinterpret_cast<const U16x8*>(
+                        kt + (32 * tb + col) * K_LD + 16 * c + 8 * half);
+                    sc[tb] = mfma_32x32x16<T>(kk, qv[c], sc[tb]);
+                }
+            const int left = k1 - k0 - i * BK;
+            if (left < BK) {
+#pragma unroll
+                for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (32 * tb + 8 * (v >> 2) + 4 * half + (v & 3) >= left)
+                            sc[tb][v] = -INFINITY;
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) mx[v & 3] = fmaxf(mx[v & 3], sc[tb][v]);
+            const float cm =
+                pair_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))) * a.scale_log2;
+            const bool grow = cm > m_run + kSlack;  // also: first finite maximum
+            float alpha = 1.f;
+            if (grow) {
+                alpha = __builtin_amdgcn_exp2f(m_run - cm);
+                m_run = cm;
+            }
+            if (__builtin_amdgcn_ballot_w64(grow)) {
+                l_run *= alpha;
+#pragma unroll
+                for (int n = 0; n < ND; ++n) o[n] *= alpha;
+            }
+            const float m_use = m_run == -INFINITY ? 0.f : m_run - kShift;
+            U16x8 pb[2 * TB];  // P, step st: token 16st + 8jj + 4*half + i at k = 4jj + i
+            float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                for (int sh = 0; sh < 2; ++sh)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float p0 = __builtin_amdgcn_exp2f(
+                            __builtin_fmaf(sc[tb][8 * sh + 2 * e], a.scale_log2, -m_use));
+                        const float p1 = __builtin_amdgcn_exp2f(
+                            __builtin_fmaf(sc[tb][8 * sh + 2 * e + 1], a.scale_log2, -m_use));
+                        const uint32_t hw = pack2<_Float16>(p0, p1);
+                        pb[2 * tb + sh].w[e] = hw;
+                        // The denominator sums the fp16 weights that P.V uses.
+                        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+                        const h2 ones = {1.f16, 1.f16};
+                        ps[e] = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, hw), ones, ps[e],
+                                                       false);
+                    }
+            l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+            const int sub = (lane >> 4) & 1;  // which 16 dims this lane's block reads
+            const uint16_t* const vl =
+                vt + (4 * half + ((lane & 15) >> 2)) * V_LD + 16 * sub + 4 * (lane & 3);
+#pragma unroll
+            for (int st = 0; st < 2 * TB; ++st)
+#pragma unroll
+                for (int n = 0; n < ND; ++n) {
+                    const uint2 lo = read_transposed(vl + (16 * st) * V_LD + 32 * n);
+                    const uint2 hi = read_transposed(vl + (16 * st + 8) * V_LD + 32 * n);
+                    const U16x8 va = {{lo.x, lo.y, hi.x, hi.y}};
+                    o[n] = mfma_32x32x16<_Float16>(va, pb[st], o[n]);
+                }
+        }
+
+        bool again = false;
+        if constexpr (kConvert) {
+            float total = 0.f;  // inf or NaN if any accumulator is
+#pragma unroll
+            for (int n = 0; n < ND; ++n)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) total += o[n][v];
+            again = !(__builtin_fabsf(total) < INFINITY);
+        }
+        // Every wave is past its reads of LDS behind this.
+        if (__syncthreads_or(again)) return true;
+        const float l = pair_sum(l_run);
+        if (qi >= q_count) return false;
+        bool direct;
+        const int64_t entry = entry_of(row, head, direct);
+        if (direct) {
+            const float inv = a.v_scale / l;
+            T* orow = a.out + a.rows[row] * a.ots + head * a.ohs + 4 * half;
+#pragma unroll
+            for (int n = 0; n < ND; ++n)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    if (32 * n + 8 * g < D) {
+                        uint2 w;
+                        w.x = pack2<T>(o[n][4 * g] * inv, o[n][4 * g + 1] * inv);
+                        w.y = pack2<T>(o[n][4 * g + 2] * inv, o[n][4 * g + 3] * inv);
+                        *reinterpret_cast<uint2*>(orow + 32 * n + 8 * g) = w;
+                    }
+        } else {
+            float* prow = a.part_o + entry * D + 4 * half;
+#pragma unroll
+            for (int n = 0; n < ND; ++n)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    if (32 * n + 8 * g < D)
+                        *reinterpret_cast<float4*>(prow + 32 * n + 8 * g) = make_float4(
+                            o[n][4 * g], o[n][4 * g + 1], o[n][4 * g + 2], o[n][4 * g + 3]);
+            if (half == 0)
+                a.part_ml[entry] =
+                    make_float2(m_run == -INFINITY ? m_run : m_run - kShift, l);
+        }
+        return false;
+    };
+
+    // ----------------------------------------------------------- narrow --
+    // Queries q0 .. q0 + qn - 1 (qn <= 16) of the task over its keys.
+    auto narrow = [&](int q0, int qn) {
+        constexpr int NT = DP == 256 ? 1 : DP == 128 ? 2 : 4;  // 16-token tiles per chunk
+        constexpr int CH = 16 * NT;
+        constexpr int KS = DP / 32;            // k-steps of Q.K^T
+        constexpr int E = DP / 16;             // V elements per lane and token
+        constexpr int VL = DP == 256 ? 2 : 1;  // loads that hold them
+        constexpr int VB = E * EB / VL;        // bytes of one
+        const int col = lane & 15, quad = lane >> 4;
+        f32x4 acc[E];  // query 4*quad + v, this lane's dim e
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float m_run = -INFINITY, l_run = 0.f;
+
+        const int per = ((k1 - k0 + 3) / 4 + 15) & ~15;
+        const int t_begin = k0 + wave * per, t_end = min(k1, t_begin + per);
+        if (t_begin < t_end) {
+            // This lane's dims: E * col .. (DP 256: 8 * col .. and 128 + 8 * col ..);
+            // lanes past the head's dims read dim 0 and write nothing.
+            auto dim_of = [&](int half) { return DP == 256 ? 128 * half + 8 * col : E * col; };
+            Bytes<8 * EB> kreg[NT][KS];
+            Bytes<VB> vreg[NT][4][VL];
+            const uint32_t last = uint32_t(t_end - 1);
+            auto load_id = [&](int t0) {
+                return ids[2 * uint64_t(page_of(min(uint32_t(t0 + lane % CH), last)))];
+            };
+            auto resolve = [&](int t0, uint32_t id) {
+                const uint32_t t = min(uint32_t(t0 + lane % CH), last);
+                return slot_of(id, t, page_of(t));
+            };
+            auto load_k = [&](uint32_t slot) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const uint32_t s = uint32_t(__shfl(int(slot), 16 * j + col, 64));
+                    const char* p = kbase + uint64_t(s) * row_bytes;
+#pragma unroll
+                    for (int c = 0; c < KS; ++c) {
+                        const int d = 32 * c + 8 * quad;
+                        kreg[j][c] = load_bytes<8 * EB>(p + (d < D ? d : 0) * EB);
+                    }
+                }
+            };
+            auto load_v = [&](uint32_t slot) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t s = uint32_t(__shfl(int(slot), 16 * j + 4 * quad + i, 64));
+                        const char* p = vbase + uint64_t(s) * row_bytes;
+#pragma unroll
+                        for (int x = 0; x < VL; ++x) {
+                            const int d = dim_of(x);
+                            vreg[j][i][x] = load_bytes<VB>(p + (d < D ? d : 0) * EB);
+                        }
+                    }
+            };
+
+            uint32_t id = load_id(t_begin);
+            U16x8 qb[KS];  // B operand: query col, dims 32c + 8*quad ..
+            {
+                int row, head;
+                query(q0 + min(col, qn - 1), row, head);
+                const T* qrow = a.q + a.rows[row] * a.qts + head * a.qhs;
+#pragma unroll
+                for (int c = 0; c < KS; ++c) {
+                    const int d = 32 * c + 8 * quad;
+                    qb[c] = d < D ? *reinterpret_cast<const U16x8*>(qrow + d) : U16x8{};
+                }
+            }
+            {
+                const uint32_t slot = resolve(t_begin, id);
+                id = load_id(t_begin + CH);
+                load_k(slot);
+                load_v(slot);
+            }
+            for (int t0 = t_begin; t0 < t_end; t0 += CH) {
+                const uint32_t next = resolve(t0 + CH, id);
+                id = load_id(t0 + 2 * CH);
+
+                float s[NT][4];  // token 16j + 4*quad + i, query col
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < KS; ++c) {
+                        U16x8 kk;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            if constexpr (F8)
+                                kk.w[w] = (w & 1) ? widen2<T, true>(kreg[j][c].w[w >> 1])
+                                                  : widen2<T, false>(kreg[j][c].w[w >> 1]);
+                            else
+                                kk.w[w] = kreg[j][c].w[w];
+                        }
+                        // Dims past the head's: zeros on both sides.
+                        if (D < DP && 32 * c + 8 * quad >= D) kk = U16x8{};
+                        d = mfma32<T>(kk, qb[c], d);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int t = t0 + 16 * j + 4 * quad + i;
+                        s[j][i] = t < t_end ? d[i] * a.scale_log2 : -INFINITY;
+                    }
+                }
+                load_k(next);
+
+                float cmax = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) cmax = fmaxf(cmax, s[j][i]);
+                cmax = fmaxf(cmax, __shfl_xor(cmax, 16, 64));
+                cmax = fmaxf(cmax, __shfl_xor(cmax, 32, 64));
+                const float m_new = fmaxf(m_run, cmax);
+                const float m_use = m_new == -INFINITY ? 0.f : m_new;
+                const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+                m_run = m_new;
+                float pw[NT][4];
+                float psum = 0.f;
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        pw[j][i] = __builtin_amdgcn_exp2f(s[j][i] - m_use);
+                        psum += pw[j][i];
+                    }
+                l_run = l_run * alpha + psum;
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const float av = __shfl(alpha, 4 * quad + v, 64);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e][v] *= av;
+                }
+                // Rows past the end hold the last token again: their weight is
+                // 0, but 0 * inf is not.
+                if (t0 + CH > t_end) {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (t0 + 16 * j + 4 * quad + i >= t_end)
+#pragma unroll
+                                for (int x = 0; x < VL; ++x) vreg[j][i][x] = Bytes<VB>{};
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    // P as a rounded value and its rounded remainder: 16 bits of
+                    // it in bf16, 22 in fp16 (weights from 2^-14 of the largest).
+                    uint2 pa, pl;
+                    pa.x = pack2<T>(pw[j][0], pw[j][1]);
+                    pa.y = pack2<T>(pw[j][2], pw[j][3]);
+                    pl.x = pack2<T>(pw[j][0] - half_lo<T>(pa.x), pw[j][1] - half_hi<T>(pa.x));
+                    pl.y = pack2<T>(pw[j][2] - half_lo<T>(pa.y), pw[j][3] - half_hi<T>(pa.y));
+                    uint32_t vw[4][E / 2];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int w = 0; w < E / 2; ++w) {
+                            constexpr int WPL = E / 2 / VL;  // T words per load
+                            const Bytes<VB>& b = vreg[j][i][w / WPL];
+                            if constexpr (F8)
+                                vw[i][w] = (w & 1) ? widen2<T, true>(b.w[(w % WPL) >> 1])
+                                                   : widen2<T, false>(b.w[(w % WPL) >> 1]);
+                            else
+                                vw[i][w] = b.w[w % WPL];
+                        }
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;
+                        uint2 vb;  // element e of tokens 4*quad + 0..3
+                        vb.x = __builtin_amdgcn_perm(vw[1][e >> 1], vw[0][e >> 1], sel);
+                        vb.y = __builtin_amdgcn_perm(vw[3][e >> 1], vw[2][e >> 1], sel);
+                        acc[e] = mfma_16x16x16<T>(pl, vb, acc[e]);
+                        acc[e] = mfma_16x16x16<T>(pa, vb, acc[e]);
+                    }
+                }
+                load_v(next);
+            }
+        }
+        l_run += __shfl_xor(l_run, 16, 64);
+        l_run += __shfl_xor(l_run, 32, 64);
+
+        // The waves' parts, merged through LDS.
+        float* const so = reinterpret_cast<float*>(lds);                 // [4][16][DP]
+        float2* const sml = reinterpret_cast<float2*>(so + 4 * kNarrow * DP);  // [4][16]
+        __syncthreads();  // a repeated call: the last one's reads are done
+        if (quad == 0) sml[wave * kNarrow + col] = make_float2(m_run, l_run);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const int h = 4 * quad + v;
+            if (h < qn) {
+                float* dst = so + (wave * kNarrow + h) * DP;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const int d = DP == 256 ? 128 * (e / 8) + 8 * col + e % 8 : E * col + e;
+                    dst[d] = acc[e][v];
+                }
+            }
+        }
+        __syncthreads();
+        constexpr int Q4 = DP / 4;
+        for (int x = tid; x < qn * Q4; x += kThreads) {
+            const int h = x / Q4, d = 4 * (x % Q4);
+            if (d >= D) continue;
+            float2 ml[4];
+            float mx = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                ml[w] = sml[w * kNarrow + h];
+                mx = fmaxf(mx, ml[w].x);
+            }
+            const float m_use = mx == -INFINITY ? 0.f : mx;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            float l = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = __builtin_amdgcn_exp2f(ml[w].x - m_use);
+                const float4 p = *reinterpret_cast<const float4*>(so + (w * kNarrow + h) * DP + d);
+                l += f * ml[w].y;
+                sum.x += f * p.x;
+                sum.y += f * p.y;
+                sum.z += f * p.z;
+                sum.w += f * p.w;
+            }
+            int row, head;
+            query(q0 + h, row, head);
+            bool direct;
+            const int64_t entry = entry_of(row, head, direct);
+            if (direct) {
+                const float inv = a.v_scale / l;
+                uint2 w;
+                w.x = pack2<T>(sum.x * inv, sum.y * inv);
+                w.y = pack2<T>(sum.z * inv, sum.w * inv);
+                *reinterpret_cast<uint2*>(a.out + a.rows[row] * a.ots + head * a.ohs + d) = w;
+            } else {
+                *reinterpret_cast<float4*>(a.part_o + entry * D + d) = sum;
+                if (d == 0) a.part_ml[entry] = make_float2(mx, l);
+            }
+        }
+    };
+
+    if (q_count > kNarrow && !wide()) return;
+    for (int q0 = 0; q0 < q_count; q0 += kNarrow) narrow(q0, min(kNarrow, q_count - q0));
+}
+
+// out = v_scale * sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the parts
+// of a (row, head), DP / 4 lanes each; rows without keys are zeros, rows of one
+// part are already written.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads)
+shared_prefix_merge(Args<T> a) {
+    constexpr int LPH = DP / 4;
+    const int32_t* const plan = a.plan;
+    if (plan[H_ROWS] != a.num_rows || plan[H_HEADS] != a.heads || plan[H_DIM] != a.head_dim ||
+        plan[H_PARTS] > a.entries)
+        return;
+    const int64_t item = (int64_t(blockIdx.x) * kThreads + threadIdx.x) / LPH;
+    if (item >= int64_t(a.num_rows) * a.heads) return;
+    const int r = int(item / a.heads), h = int(item - int64_t(r) * a.heads);
+    const int d = 4 * int(threadIdx.x % LPH);
+    const int parts = plan[a.rows_at + 2 * r + 1];
+    if (d >= a.head_dim || parts == 1) return;
+    const int64_t first = int64_t(plan[a.rows_at + 2 * r]) * a.heads + h;
+    float mx = -INFINITY;
+    for (int s = 0; s < parts; ++s) mx = fmaxf(mx, a.part_ml[first + int64_t(s) * a.heads].x);
+    const float m_use = mx == -INFINITY ? 0.f : mx;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < parts; ++s) {
+        const int64_t e = first + int64_t(s) * a.heads;
+        const float2 ml = a.part_ml[e];
+        const float4 p = *reinterpret_cast<const float4*>(a.part_o + e * a.head_dim + d);
+        const float f = __builtin_amdgcn_exp2f(ml.x - m_use);
+        l += f * ml.y;
+        sum.x += f * p.x;
+        sum.y += f * p.y;
+        sum.z += f * p.z;
+        sum.w += f * p.w;
+    }
+    const float inv = parts == 0 ? 0.f : a.v_scale / l;
+    uint2 w;
+    w.x = pack2<T>(sum.x * inv, sum.y * inv);
+    w.y = pack2<T>(sum.z * inv, sum.w * inv);
+    *reinterpret_cast<uint2*>(a.out + a.rows[r] * a.ots + h * a.ohs + d) = w;
+}
+
+int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+bool plan_geometry_ok(int64_t max_rows, int64_t heads, int64_t kv_heads) {
+    // (so that a plan's words and its parts' numbers fit in 32 bits)
+    return max_rows > 0 && max_rows <= (1 << 20) && heads > 0 && heads <= (1 << 12) &&
+           max_rows * heads <= (1 << 26) && kv_heads > 0 && heads % kv_heads == 0;
+}
+
+}  // namespace
+}  // namespace tvllm
+
+using namespace tvllm;
+
+extern "C" int64_t tvllm_shared_prefix_plan_words(int64_t max_rows, int64_t num_heads,
+                                                  int64_t num_kv_heads) {
+    if (!plan_geometry_ok(max_rows, num_heads, num_kv_heads)) return 0;
+    return plan_layout(max_rows, num_heads, num_kv_heads).words;
+}
+
+extern "C" int64_t tvllm_shared_prefix_max_tasks(int64_t max_rows, int64_t num_heads,
+                                                 int64_t num_kv_heads) {
+    if (!plan_geometry_ok(max_rows, num_heads, num_kv_heads)) return 0;
+    return plan_layout(max_rows, num_heads, num_kv_heads).max_tasks;
+}
+
+extern "C" int64_t tvllm_shared_prefix_workspace_size(int64_t max_rows, int64_t num_heads,
+                                                      int64_t num_kv_heads, int64_t head_dim) {
+    if (!plan_geometry_ok(max_rows, num_heads, num_kv_heads) || head_dim <= 0) return 0;
+    return max_entries(max_rows, num_heads) * (head_dim + 2) * 4;
+}
+
+extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* groups,
+                                        const int64_t* prefix_lens, int64_t num_rows,
+                                        int64_t num_groups, int64_t max_rows, int64_t num_heads,
+                                        int64_t num_kv_heads, int64_t head_dim,
+                                        int64_t block_size, int32_t* plan, int64_t plan_words,
+                                        int64_t* num_tasks, int64_t* workspace_bytes) {
+    TVLLM_CHECK(plan_geometry_ok(max_rows, num_heads, num_kv_heads),
+                "shared_prefix_plan: invalid geometry");
+    TVLLM_CHECK(head_dim > 0 && head_dim <= 256 && head_dim % 8 == 0,
+                "shared_prefix_plan: head_dim must be a multiple of 8 up to 256");
+    TVLLM_CHECK(block_size > 0 && block_size <= INT32_MAX, "shared_prefix_plan: invalid block size");
+    TVLLM_CHECK(num_rows >= 0 && num_rows <= max_rows && num_groups >= 0,
+                "shared_prefix_plan: more rows than the plan holds");
+    const PlanLayout lay = plan_layout(max_rows, num_heads, num_kv_heads);
+    TVLLM_CHECK(plan && num_tasks && workspace_bytes && plan_words >= lay.words,
+                "shared_prefix_plan: the plan buffer is too small");
+    TVLLM_CHECK(num_rows == 0 || (lengths && groups), "shared_prefix_plan: null pointer");
+    TVLLM_CHECK(num_groups == 0 || prefix_lens, "shared_prefix_plan: null pointer");
+    for (int64_t g = 0; g < num_groups; ++g)
+        TVLLM_CHECK(prefix_lens[g] >= 0 && prefix_lens[g] <= INT32_MAX &&
+                        prefix_lens[g] % block_size == 0,
+                    "shared_prefix_plan: prefix lengths must be whole blocks");
+    const int64_t group = num_heads / num_kv_heads;
+    struct Group {
+        int64_t count = 0, first = 0, prefix = 0, splits = 0, per = 0;
+    };
+    try {
+        std::vector<Group> gs(static_cast<size_t>(num_groups));
+        for (int64_t r = 0; r < num_rows; ++r) {
+            TVLLM_CHECK(lengths[r] >= 0 && lengths[r] <= INT32_MAX,
+                        "shared_prefix_plan: invalid context length");
+            TVLLM_CHECK(groups[r] >= -1 && groups[r] < num_groups,
+                        "shared_prefix_plan: group index out of range");
+            if (groups[r] < 0) continue;
+            TVLLM_CHECK(lengths[r] >= prefix_lens[groups[r]],
+                        "shared_prefix_plan: a row is shorter than its group's prefix");
+            ++gs[groups[r]].count;
+        }
+        // Members: the groups' rows side by side, then the others. A prefix
+        // that only one row has is that row's own keys.
+        int64_t at = 0;
+        for (int64_t g = 0; g < num_groups; ++g) {
+            gs[g].first = at;
+            at += gs[g].count;
+            gs[g].prefix = gs[g].count > 1 ? prefix_lens[g] : 0;
+        }
+        std::vector<int64_t> next(static_cast<size_t>(num_groups)), place(static_cast<size_t>(num_rows)),
+            own(static_cast<size_t>(num_rows));
+        for (int64_t g = 0; g < num_groups; ++g) next[g] = gs[g].first;
+        int32_t* const rows = plan + lay.rows_at;
+        int32_t* const members = plan + lay.members_at;
+        int32_t* const tasks = plan + lay.tasks_at;
+        int64_t cost = 0;
+        const int64_t own_tiles = div_up(group, kWide);
+        for (int64_t r = 0; r < num_rows; ++r) {
+            const int64_t g = groups[r];
+            place[r] = g >= 0 ? next[g]++ : at++;
+            members[place[r]] = int32_t(r);
+            own[r] = lengths[r] - (g >= 0 ? gs[g].prefix : 0);
+            cost += own_tiles * num_kv_heads * own[r];
+        }
+        for (const Group& g : gs) cost += div_up(g.count * group, kWide) * num_kv_heads * g.prefix;
+        const int64_t chunk =
+            std::max(kMinKeys, div_up(div_up(cost, kTargetTasks), kKeyUnit) * kKeyUnit);
+        auto cut = [&](int64_t keys, int64_t& splits, int64_t& per) {
+            splits = std::min(kMaxParts, div_up(keys, chunk));
+            per = splits ? div_up(div_up(keys, splits), kKeyUnit) * kKeyUnit : 0;
+            if (per) splits = div_up(keys, per);
+        };
+        int64_t n = 0;
+        auto emit = [&](int64_t member, int64_t q0, int64_t count, int64_t kvh, int64_t k0,
+                        int64_t k1, int64_t part) {
+            int32_t* t = tasks + n++ * kTaskWords;
+            t[T_MEMBER] = int32_t(member);
+            t[T_QBEGIN] = int32_t(q0);
+            t[T_QCOUNT] = int32_t(count);
+            t[T_KVH] = int32_t(kvh);
+            t[T_K0] = int32_t(k0);
+            t[T_K1] = int32_t(k1);
+            t[T_PART] = int32_t(part);
+            t[T_UNUSED] = 0;
+        };
+        // Shared keys first, the longest tasks ahead. Workgroups are dealt to
+        // the 8 XCDs in turn: the query tiles of one (KV head, range of keys)
+        // go 8 apart, onto one XCD, whose L2 they share.
+        struct Column {
+            int64_t g, kvh, split;
+        };
+        std::vector<int64_t> order;
+        for (int64_t g = 0; g < num_groups; ++g) {
+            cut(gs[g].prefix, gs[g].splits, gs[g].per);
+            if (gs[g].splits) order.push_back(g);
+        }
+        std::sort(order.begin(), order.end(), [&](int64_t x, int64_t y) {
+            return gs[x].per != gs[y].per ? gs[x].per > gs[y].per : x < y;
+        });
+        std::vector<Column> columns;
+        for (int64_t g : order) {
+            columns.clear();
+            for (int64_t s = 0; s < gs[g].splits; ++s)
+                for (int64_t h = 0; h < num_kv_heads; ++h) columns.push_back({g, h, s});
+            const int64_t queries = gs[g].count * group, tiles = div_up(queries, kWide);
+            const int64_t tile = div_up(div_up(queries, tiles), 32) * 32;
+            for (size_t c0 = 0; c0 < columns.size(); c0 += 8)
+                for (int64_t t = 0; t < tiles; ++t)
+                    for (size_t c = c0; c < std::min(columns.size(), c0 + 8); ++c) {
+                        const int64_t k0 = columns[c].split * gs[g].per;
+                        const int64_t q0 = t * tile;
+                        if (q0 < queries)
+                            emit(gs[g].first, q0, std::min(tile, queries - q0), columns[c].kvh, k0,
+                                 std::min(gs[g].prefix, k0 + gs[g].per), columns[c].split);
+                    }
+        }
+        order.resize(static_cast<size_t>(num_rows));
+        for (int64_t r = 0; r < num_rows; ++r) order[r] = r;
+        std::sort(order.begin(), order.end(), [&](int64_t x, int64_t y) {
+            return own[x] != own[y] ? own[x] > own[y] : x < y;
+        });
+        std::vector<int64_t> parts(static_cast<size_t>(num_rows));
+        for (int64_t r : order) {
+            const int64_t g = groups[r], shared = g >= 0 ? gs[g].splits : 0;
+            const int64_t begin = g >= 0 ? gs[g].prefix : 0;
+            int64_t splits, per;
+            cut(own[r], splits, per);
+            parts[r] = shared + splits;
+            for (int64_t s = 0; s < splits; ++s)
+                for (int64_t t = 0; t < own_tiles; ++t)
+                    for (int64_t h = 0; h < num_kv_heads; ++h) {
+                        const int64_t k0 = begin + s * per;
+                        emit(place[r], t * kWide, std::min<int64_t>(kWide, group - t * kWide), h,
+                             k0, std::min(lengths[r], k0 + per), shared + s);
+                    }
+        }
+        int64_t entries = 0;
+        for (int64_t r = 0; r < num_rows; ++r) {
+            rows[2 * r] = int32_t(entries);
+            rows[2 * r + 1] = int32_t(parts[r]);
+            if (parts[r] > 1) entries += parts[r];
+        }
+        std::fill(plan, plan + kHeader, 0);
+        plan[H_TASKS] = int32_t(n);
+        plan[H_ROWS] = int32_t(num_rows);
+        plan[H_HEADS] = int32_t(num_heads);
+        plan[H_KV_HEADS] = int32_t(num_kv_heads);
+        plan[H_DIM] = int32_t(head_dim);
+        plan[H_BLOCK] = int32_t(block_size);
+        plan[H_PARTS] = int32_t(entries * num_heads);
+        *num_tasks = n;
+        *workspace_bytes = entries * num_heads * (head_dim + 2) * 4;
+        clear_error();
+        return TVLLM_OK;
+    } catch (const std::exception&) {  // no memory for the lists
+        set_error("shared_prefix_plan: out of host memory");
+        return TVLLM_EINVAL;
+    }
+}
+
+extern "C" int tvllm_paged_decode_shared_prefix(
+    const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+    const void* v_cache, void* out, int64_t out_token_stride, int64_t out_head_stride,
+    const int64_t* rows, const int64_t* blocks, const int64_t* offsets, const int32_t* plan,
+    int64_t num_rows, int64_t max_rows, int64_t num_tasks, int64_t num_heads,
+    int64_t num_kv_heads, int64_t head_dim, int64_t num_slots, int64_t cache_slot_stride,
+    int64_t cache_head_stride, int64_t block_size, float scale, void* workspace,
+    int64_t workspace_bytes, int dtype, int cache_dtype, float k_scale, float v_scale,
+    tvllm_stream_t stream) {
+    const bool f8 = cache_dtype == TVLLM_FP8_E4M3;
+    TVLLM_CHECK(dtype == TVLLM_BF16 || dtype == TVLLM_F16,
+                "shared_prefix: Q must be float16 or bfloat16");
+    TVLLM_CHECK(f8 || cache_dtype == dtype,
+                "shared_prefix: KV cache dtype must match Q or be FP8 E4M3");
+    TVLLM_CHECK(k_scale > 0.f && v_scale > 0.f && k_scale < INFINITY && v_scale < INFINITY,
+                "shared_prefix: KV scales must be positive and finite");
+    TVLLM_CHECK(f8 || (k_scale == 1.f && v_scale == 1.f),
+                "shared_prefix: KV scales apply to an FP8 cache only");
+    TVLLM_CHECK(plan_geometry_ok(max_rows, num_heads, num_kv_heads),
+                "shared_prefix: invalid GQA geometry");
+    TVLLM_CHECK(head_dim > 0 && head_dim <= 256 && head_dim % 8 == 0,
+                "shared_prefix: head_dim must be a multiple of 8 up to 256");
+    TVLLM_CHECK(block_size > 0 && num_slots > 0 && num_slots % block_size == 0,
+                "shared_prefix: invalid block geometry");
+    TVLLM_CHECK(num_slots <= INT32_MAX, "shared_prefix: at most 2^31-1 cache slots");
+    TVLLM_CHECK(cache_layout_ok(num_slots, num_kv_heads, head_dim, cache_slot_stride,
+                                cache_head_stride),
+                "shared_prefix: cache strides must give non-overlapping head rows");
+    TVLLM_CHECK(scale > 0.f && scale < INFINITY, "shared_prefix: scale must be positive");
+    TVLLM_CHECK(num_rows >= 0 && num_rows <= max_rows && workspace_bytes >= 0,
+                "shared_prefix: negative sizes, or more rows than the plan holds");
+    const PlanLayout lay = plan_layout(max_rows, num_heads, num_kv_heads);
+    TVLLM_CHECK(num_tasks >= 0 && num_tasks <= lay.max_tasks,
+                "shared_prefix: more tasks than the plan holds");
+    if (num_rows == 0) {
+        clear_error();
+        return TVLLM_OK;
+    }
+    TVLLM_CHECK(q && k_cache && v_cache && out && rows && blocks && offsets && plan,
+                "shared_prefix: null pointer");
+    TVLLM_CHECK(workspace || workspace_bytes == 0, "shared_prefix: null workspace");
+    TVLLM_CHECK(cache_slot_stride % 8 == 0 && cache_head_stride % 8 == 0 &&
+                    cache_slot_stride * (f8 ? 1 : 2) <= int64_t(UINT32_MAX) &&
+                    (f8 ? aligned8(k_cache) && aligned8(v_cache)
+                        : aligned16(k_cache) && aligned16(v_cache)),
+                "shared_prefix: cache rows must be whole, aligned 8-element units "
+                "(slot stride below 2^32 bytes)");
+    TVLLM_CHECK(aligned16(q) && q_token_stride % 8 == 0 && q_head_stride % 8 == 0,
+                "shared_prefix: Q rows must be 16-byte aligned");
+    TVLLM_CHECK(aligned8(out) && out_token_stride % 4 == 0 && out_head_stride % 4 == 0,
+                "shared_prefix: output rows must be 8-byte aligned");
+    TVLLM_CHECK(aligned16(workspace), "shared_prefix: the workspace must be 16-byte aligned");
+    hipStream_t s = as_hip(stream);
+    return dispatch_half(dtype, [&]<int DT>() {
+        using T = typename Elem<DT>::T;
+        Args<T> a{};
+        a.q = static_cast<const T*>(q);
+        a.qts = q_token_stride;
+        a.qhs = q_head_stride;
+        a.k = k_cache;
+        a.v = v_cache;
+        a.css = cache_slot_stride;
+        a.chs = cache_head_stride;
+        a.out = static_cast<T*>(out);
+        a.ots = out_token_stride;
+        a.ohs = out_head_stride;
+        a.rows = rows;
+        a.blocks = blocks;
+        a.offsets = offsets;
+        a.plan = plan;
+        a.rows_at = int(lay.rows_at);
+        a.members_at = int(lay.members_at);
+        a.tasks_at = int(lay.tasks_at);
+        a.num_rows = int(num_rows);
+        a.heads = int(num_heads);
+        a.kv_heads = int(num_kv_heads);
+        a.group = int(num_heads / num_kv_heads);
+        a.head_dim = int(head_dim);
+        a.block_size = int(block_size);
+        // With 2^(s-1) < d <= 2^s, m = ceil(2^(31+s) / d) fits in 32 bits and
+        // (t m) >> (31 + s) is t / d for every t < 2^31.
+        int sh = 0;
+        while ((int64_t(1) << sh) < block_size) ++sh;
+        a.page_shift = 31 + sh;
+        a.page_mul = uint32_t(((uint64_t(1) << a.page_shift) + uint64_t(block_size) - 1) /
+                              uint64_t(block_size));
+        a.scale_log2 = scale * kLog2e * k_scale;
+        a.v_scale = v_scale;
+        a.entries = workspace_bytes / ((head_dim + 2) * 4);
+        a.part_o = static_cast<float*>(workspace);
+        a.part_ml = reinterpret_cast<float2*>(a.part_o + a.entries * head_dim);
+        auto go = [&]<int DP>() {
+            if (num_tasks) {
+                if (f8) shared_prefix_tasks<T, DP, true><<<int(num_tasks), kThreads, 0, s>>>(a);
+                else shared_prefix_tasks<T, DP, false><<<int(num_tasks), kThreads, 0, s>>>(a);
+            }
+            const int64_t threads = num_rows * num_heads * (DP / 4);
+            shared_prefix_merge<T, DP>
+                <<<int((threads + kThreads - 1) / kThreads), kThreads, 0, s>>>(a);
+        };
+        if (head_dim <= 32) go.template operator()<32>();
+        else if (head_dim <= 64) go.template operator()<64>();
+        else if (head_dim <= 128) go.template operator()<128>();
+        else go.template operator()<256>();
+        return launch_status("shared_prefix");
+    });
+}

@@ -56,6 +56,14 @@ _SIGNATURES: dict[str, tuple[type, list[type]]] = {
         _INT, [_P, _I64, _I64, _P, _P, _P, _P, _F32, _F32, _P, _P, _P, _P, _I64, _I64, _P,
                _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F32, _P,
                _I64, _INT, _INT, _F32, _F32, _P]),
+    "tvllm_shared_prefix_plan_words": (_I64, [_I64] * 3),
+    "tvllm_shared_prefix_max_tasks": (_I64, [_I64] * 3),
+    "tvllm_shared_prefix_workspace_size": (_I64, [_I64] * 4),
+    "tvllm_shared_prefix_plan": (_INT, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                                        _P, _I64, _P, _P]),
+    "tvllm_paged_decode_shared_prefix": (
+        _INT, [_P, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
+               _I64, _I64, _I64, _I64, _I64, _I64, _F32, _P, _I64, _INT, _INT, _F32, _F32, _P]),
     "tvllm_few_rows_linear": (_INT, [_P, _I64, _P, _I64, _I64, _I64, _P, _I64, _INT, _INT, _P]),
     "tvllm_rms_norm": (_INT, [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64,
                               _P, _P, _F32, _INT, _P]),

@@ -405,6 +405,36 @@ int tvllm_argmax(const void* logits, int64_t rows, int64_t vocab,
                  int64_t row_stride, int64_t* out, int dtype,
                  tvllm_stream_t stream);
 
+/* Logit controls in front of the sampler, for row r and token i, in fp32:
+ *   seen:  x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   x = x - frequency[r] * c - presence[r] * [c > 0]
+ *   x = x + bias_values[j], j the last of bias_offsets[r] .. bias_offsets[r + 1]
+ *     - 1 with bias_tokens[j] == i
+ *   x = -inf where bit i % 32 of mask[mask_rows[r] * mask_stride + i / 32] is 0
+ * rounded once to out_dtype (dtype or TVLLM_F32). The row's history is
+ * history[slots[r] * capacity + p], p < lengths[r] (at most capacity): i is
+ * seen if it stands there, c counts it at p >= prompt_lens[r]. newest, where
+ * given, holds the token of position lengths[r] - 1, which the call writes
+ * into the history (no other row then reads that slot). Null history: no
+ * penalties; null repetition / presence / frequency: 1 / 0 / 0; null newest,
+ * bias_offsets, mask_rows: none. A slot outside [0, num_slots), a mask row
+ * outside [0, mask_count), ids outside [0, vocab) count as none; bias offsets
+ * are held to [0, num_bias]. logits and out: [rows, vocab] with row strides of
+ * at least vocab, the same tensor or disjoint ones.
+ * No counterpart in the reference (tinyvllm/sampling.py:21-72 samples from the
+ * logits as they are). */
+int tvllm_logit_controls(const void* logits, int64_t rows, int64_t vocab,
+                         int64_t row_stride, const float* repetition,
+                         const float* presence, const float* frequency,
+                         int32_t* history, int64_t num_slots, int64_t capacity,
+                         const int64_t* slots, const int64_t* lengths,
+                         const int64_t* prompt_lens, const int64_t* newest,
+                         const int32_t* bias_tokens, const float* bias_values,
+                         const int64_t* bias_offsets, int64_t num_bias,
+                         const int32_t* mask, int64_t mask_count, int64_t mask_stride,
+                         const int64_t* mask_rows, void* out, int64_t out_stride,
+                         int dtype, int out_dtype, tvllm_stream_t stream);
+
 /* Temperature / top-k / top-p sampling by the exponential race:
  *   s = (logit - max) / temperature;  keep the top_k largest (0 = all);
  *   keep the smallest prefix of the descending order whose probability

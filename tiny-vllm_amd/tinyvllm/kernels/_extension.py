@@ -74,6 +74,9 @@ _SIGNATURES: dict[str, tuple[type, list[type]]] = {
                                   _P, _I64, _I64, _I64, _I64, _F32, _F32, _P,
                                   _P, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64,
                                   _INT, _INT, _F32, _F32, _P]),
+    "tvllm_logit_controls": (_INT, [_P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _P, _P, _P,
+                                    _P, _P, _P, _P, _I64, _P, _I64, _I64, _P, _P, _I64, _INT,
+                                    _INT, _P]),
     "tvllm_argmax": (_INT, [_P, _I64, _I64, _I64, _P, _INT, _P]),
     "tvllm_sample_workspace_size": (_I64, [_I64, _I64]),
     "tvllm_sample_split_workspace_size": (_I64, [_I64, _I64]),

@@ -1,0 +1,119 @@
+"""Logit controls in front of the sampler: penalties, biases and token masks
+(no reference counterpart: the reference samples from the logits as they are,
+tinyvllm/sampling.py:21-72)."""
+from __future__ import annotations
+
+import torch
+
+from tinyvllm.kernels._extension import (
+    check, dtype_code, load_kernels, require_gpu, stream_of,
+)
+from tinyvllm.kernels.sampling import _check_logits
+
+
+def _ptr(tensor: torch.Tensor | None) -> int | None:
+    return None if tensor is None or tensor.numel() == 0 else tensor.data_ptr()
+
+
+def apply_logit_controls(
+    logits: torch.Tensor,
+    *,
+    repetition: torch.Tensor | None = None,
+    presence: torch.Tensor | None = None,
+    frequency: torch.Tensor | None = None,
+    history: torch.Tensor | None = None,
+    slots: torch.Tensor | None = None,
+    lengths: torch.Tensor | None = None,
+    prompt_lens: torch.Tensor | None = None,
+    newest: torch.Tensor | None = None,
+    bias_tokens: torch.Tensor | None = None,
+    bias_values: torch.Tensor | None = None,
+    bias_offsets: torch.Tensor | None = None,
+    mask: torch.Tensor | None = None,
+    mask_rows: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Each row's controls applied to its logits [rows, vocab], in this order:
+
+    * tokens in the row's history: positive logits divided by ``repetition[r]``,
+      others multiplied by it; then ``frequency[r]`` times the number of times
+      the token stands in the answer part subtracted, and ``presence[r]`` if
+      it stands there (float32 [rows]; None: 1, 0 and 0);
+    * ``bias_values[j]`` added to token ``bias_tokens[j]`` for
+      ``bias_offsets[r] <= j < bias_offsets[r + 1]`` (int32, float32, int64
+      [rows + 1]); of a token that a row lists twice the last entry counts;
+    * tokens whose bit in ``mask[mask_rows[r]]`` is 0 set to -inf (token i: bit
+      i % 32 of word i // 32; int32 [masks, words], int64 [rows], -1: no mask).
+
+    ``history`` (int32 [slots, capacity]) holds token ids by position; row r's
+    is ``history[slots[r], :lengths[r]]`` (int64 [rows]; slot -1: none), of
+    which the first ``prompt_lens[r]`` are its prompt. ``newest`` (int64
+    [rows]), where given, is the token at position ``lengths[r] - 1``: it is
+    counted and written into the history (rows then need slots of their own).
+    Ids outside the vocabulary, slots and mask rows outside their tensors count
+    as none.
+
+    ``out`` receives the result: None for a new tensor of the logits' type, a
+    float32 or same-type tensor of their shape, or ``logits`` itself. Computed
+    in float32 and rounded once to ``out``'s type."""
+    _check_logits(logits)
+    rows, vocab = logits.shape
+    device = require_gpu(logits)
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=device)
+    elif (out.shape != logits.shape or out.stride(1) != 1
+          or out.dtype not in (logits.dtype, torch.float32)):
+        raise RuntimeError("out must be float32 or of the logits' type, of their shape, with "
+                           "unit last stride")
+    for name, tensor, dtype, size in (
+            ("repetition", repetition, torch.float32, rows),
+            ("presence", presence, torch.float32, rows),
+            ("frequency", frequency, torch.float32, rows),
+            ("slots", slots, torch.long, rows), ("lengths", lengths, torch.long, rows),
+            ("prompt_lens", prompt_lens, torch.long, rows),
+            ("newest", newest, torch.long, rows), ("mask_rows", mask_rows, torch.long, rows),
+            ("bias_offsets", bias_offsets, torch.long, rows + 1),
+            ("bias_tokens", bias_tokens, torch.int32, None),
+            ("bias_values", bias_values, torch.float32, None)):
+        if tensor is None:
+            continue
+        if tensor.dtype != dtype or tensor.dim() != 1 or not tensor.is_contiguous() or (
+                size is not None and tensor.numel() != size):
+            raise RuntimeError(f"{name} must be a contiguous {dtype} vector"
+                               + ("" if size is None else f" of {size}"))
+        require_gpu(logits, tensor)
+    if history is not None:
+        if slots is None or lengths is None or prompt_lens is None:
+            raise RuntimeError("a history needs slots, lengths and prompt_lens")
+        if history.dtype != torch.int32 or history.dim() != 2 or not history.is_contiguous():
+            raise RuntimeError("history must be contiguous int32 [slots, capacity]")
+        require_gpu(logits, history)
+    elif any(t is not None for t in (repetition, presence, frequency, newest)):
+        raise RuntimeError("penalties need a history")
+    if (bias_offsets is None) != (bias_tokens is None) or (bias_tokens is None) != (
+            bias_values is None):
+        raise RuntimeError("biases need tokens, values and offsets")
+    if bias_tokens is not None and bias_tokens.numel() != bias_values.numel():
+        raise RuntimeError("bias_tokens and bias_values must align")
+    if (mask is None) != (mask_rows is None):
+        raise RuntimeError("masks need mask_rows")
+    if mask is not None:
+        if mask.dtype != torch.int32 or mask.dim() != 2 or mask.stride(1) != 1 or (
+                mask.shape[0] and mask.shape[1] < -(-vocab // 32)):
+            raise RuntimeError("mask must be int32 [masks, words] with unit last stride and a "
+                               "bit for every token")
+        require_gpu(logits, mask)
+    require_gpu(logits, out)
+    if rows == 0:
+        return out
+    check(load_kernels().tvllm_logit_controls(
+        logits.data_ptr(), rows, vocab, logits.stride(0), _ptr(repetition), _ptr(presence),
+        _ptr(frequency), _ptr(history), 0 if history is None else history.shape[0],
+        0 if history is None else history.shape[1], _ptr(slots), _ptr(lengths),
+        _ptr(prompt_lens), _ptr(newest), _ptr(bias_tokens), _ptr(bias_values),
+        _ptr(bias_offsets), 0 if bias_tokens is None else bias_tokens.numel(), _ptr(mask),
+        0 if mask is None else mask.shape[0], 0 if mask is None else mask.stride(0),
+        _ptr(mask_rows), out.data_ptr(), out.stride(0), dtype_code(logits.dtype),
+        dtype_code(out.dtype), stream_of(device),
+    ))
+    return out

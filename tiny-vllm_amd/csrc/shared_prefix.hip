@@ -109,7 +109,7 @@ struct Args {
     const int32_t* plan;
     int rows_at, members_at, tasks_at;
     int num_rows, heads, kv_heads, group, head_dim, block_size;
-    uint32_t page_mul;  // t / block_size == (t * page_mul) >> page_shift, t < 2^31
+    uint32_t page_mul;  // t / block_size == (2 t * page_mul >> 32) >> page_shift, t < 2^31
     int page_shift;
     float scale_log2;  // softmax scale * log2(e) (* k_scale for an FP8 cache)
     float v_scale;     // FP8 cache: V dequantisation scale (1 otherwise)
@@ -117,6 +117,14 @@ struct Args {
     float2* part_ml;   // [entries]: (max, sum) in base 2
     int64_t entries;   // room in the two
 };
+
+template <int I, int N, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        static_for<I + 1, N>(f);
+    }
+}
 
 __device__ __forceinline__ float as_f(uint32_t x) { return __uint_as_float(x); }
 __device__ __forceinline__ uint32_t as_u(float x) { return __float_as_uint(x); }
@@ -213,11 +221,32 @@ __device__ __forceinline__ uint32_t widen2(uint32_t w) {
     }
 }
 
+// The order of a wide step's instructions: the first operands from LDS, the
+// weights' arithmetic, then one matrix instruction at a time, each followed by
+// the read of the operand four further on and a share of the vector work.
+// Without it the compiler puts each read right before the instruction that
+// waits for it.
+template <int NC, int ND>
+__device__ __forceinline__ void interleave() {
+    constexpr int kValu = 0x2, kMfma = 0x8, kRead = 0x100;
+    constexpr int kAll = NC + 2 * ND, kAhead = 4;  // operands: K one read each, V two
+    static_for<0, kAhead>([&](auto m) {
+        __builtin_amdgcn_sched_group_barrier(kRead, m < NC ? 1 : 2, 0);
+    });
+    __builtin_amdgcn_sched_group_barrier(kValu, 20, 0);
+    static_for<0, kAll>([&](auto m) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+        if constexpr (m + kAhead < kAll)
+            __builtin_amdgcn_sched_group_barrier(kRead, m + kAhead < NC ? 1 : 2, 0);
+        __builtin_amdgcn_sched_group_barrier(kValu, 5, 0);
+    });
+}
+
 template <typename T, int DP, bool F8>
 __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2)
 shared_prefix_tasks(Args<T> a) {
     constexpr int EB = F8 ? 1 : 2;             // bytes per cached element
-    constexpr int BK = DP == 256 ? 32 : 64;    // tokens per wide tile
+    constexpr int BK = 32;                     // tokens per wide tile
     constexpr int K_LD = DP + 8;               // LDS row strides (elements): 16-byte reads
     constexpr int V_LD = DP == 32 ? 32 : DP + 32;  // and transposing reads without conflicts
     constexpr int K_TILE = BK * K_LD, V_TILE = BK * V_LD;
@@ -243,9 +272,7 @@ shared_prefix_tasks(Args<T> a) {
     const char* const kbase = static_cast<const char*>(a.k) + int64_t(kvh) * a.chs * EB;
     const char* const vbase = static_cast<const char*>(a.v) + int64_t(kvh) * a.chs * EB;
 
-    auto page_of = [&](uint32_t t) {
-        return uint32_t((uint64_t(t) * a.page_mul) >> a.page_shift);
-    };
+    auto page_of = [&](uint32_t t) { return __umulhi(2 * t, a.page_mul) >> a.page_shift; };
     auto slot_of = [&](uint32_t id, uint32_t t, uint32_t page) {
         return id * uint32_t(a.block_size) + (t - page * uint32_t(a.block_size));
     };
@@ -265,9 +292,7 @@ shared_prefix_tasks(Args<T> a) {
     // ------------------------------------------------------------- wide --
     // Returns whether the outputs are not what fp16 V can give (see below).
     auto wide = [&]() -> bool {
-        constexpr int PPR = DP / 8;               // 8-element pieces per row
-        constexpr int JP = BK * PPR / kThreads;   // pieces per thread, K and V each
-        constexpr int TB = BK / 32;
+        constexpr int PPR = DP / 8;  // 8-element pieces per row
         constexpr int NC = DP / 16, ND = DP / 32;
         constexpr int EBP = 8 * EB;
         // A bf16 cache's V enters the products as fp16 (P needs its 11 bits: a
@@ -279,8 +304,9 @@ shared_prefix_tasks(Args<T> a) {
         uint16_t* const ks = reinterpret_cast<uint16_t*>(lds);
         uint16_t* const vs = ks + 2 * K_TILE;
         const int col = lane & 31, half = lane >> 5;
+        // Waves past the queries take the last one along: a second path through
+        // the loop for them would make the others wait for its loads.
         const int qi = wave * 32 + col;
-        const bool active = wave * 32 < q_count;
         int row, head;
         query(min(qi, q_count - 1), row, head);
 
@@ -296,152 +322,244 @@ shared_prefix_tasks(Args<T> a) {
 
         const int ntiles = (k1 - k0 + BK - 1) / BK;
         const uint32_t last = uint32_t(k1 - 1);
-        uint32_t id[JP];
-        Bytes<EBP> kst[JP], vst[JP];
+        // Staging: LPR lanes side by side load a row's whole 128-byte lines
+        // (its first 64 bytes where it has fewer), each thread PT pieces of each
+        // of its JT tokens, so a page is looked up once for those. Two sets of
+        // registers, a tile each: rows are loaded two tiles ahead of the step
+        // that stores them in LDS.
+        constexpr int LPR = PPR < 8 ? PPR : 8;
+        constexpr int TSTEP = kThreads / LPR;  // tokens that one round covers
+        constexpr int JT = BK > TSTEP ? BK / TSTEP : 1, PT = PPR / LPR;
+        const int tok0 = tid / LPR, piece0 = tid % LPR;
+        struct Stage {
+            Bytes<EBP> k[JT][PT], v[JT][PT];
+            uint64_t off[JT];
+        };
+        Stage st0, st1;
+        uint32_t id[JT];
         auto token_of = [&](int i, int j) {  // past the end: the last token again
-            return min(uint32_t(k0 + i * BK + (tid + j * kThreads) / PPR), last);
+            return min(uint32_t(k0 + i * BK + tok0 + j * TSTEP), last);
         };
         auto load_ids = [&](int i) {
 #pragma unroll
-            for (int j = 0; j < JP; ++j) id[j] = ids[2 * uint64_t(page_of(token_of(i, j)))];
+            for (int j = 0; j < JT; ++j) id[j] = ids[2 * uint64_t(page_of(token_of(i, j)))];
         };
-        auto load_tile = [&](int i) {
+        auto locate = [&](Stage& st, int i) {  // tile i's rows, by the ids loaded for it
 #pragma unroll
-            for (int j = 0; j < JP; ++j) {
+            for (int j = 0; j < JT; ++j) {
                 const uint32_t t = token_of(i, j);
-                const int piece = (tid + j * kThreads) % PPR;
-                const uint64_t off = uint64_t(slot_of(id[j], t, page_of(t))) * row_bytes +
-                                     uint32_t((piece * 8 < D ? piece : 0) * EBP);
-                kst[j] = load_bytes<EBP>(kbase + off);
-                vst[j] = load_bytes<EBP>(vbase + off);
+                st.off[j] = uint64_t(slot_of(id[j], t, page_of(t))) * row_bytes;
             }
         };
-        auto store_tile = [&](int i) {
-            uint16_t* const kt = ks + (i & 1) * K_TILE;
-            uint16_t* const vt = vs + (i & 1) * V_TILE;
-            const int left = k1 - k0 - i * BK;
+        auto load = [&](Bytes<EBP> (&to)[JT][PT], const uint64_t (&off)[JT], const char* base) {
 #pragma unroll
-            for (int j = 0; j < JP; ++j) {
-                const int tok = (tid + j * kThreads) / PPR;
-                const int piece = (tid + j * kThreads) % PPR;
-                // Rows past the end and dims past the head's are zeros.
-                const bool keep = tok < left && piece * 8 < D;
-                U16x8 kw, vw;
+            for (int j = 0; j < JT; ++j)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    if constexpr (F8) {
-                        kw.w[w] = (w & 1) ? widen2<T, true>(kst[j].w[w >> 1])
-                                          : widen2<T, false>(kst[j].w[w >> 1]);
-                        vw.w[w] = (w & 1) ? widen2<_Float16, true>(vst[j].w[w >> 1])
-                                          : widen2<_Float16, false>(vst[j].w[w >> 1]);
-                    } else {
-                        kw.w[w] = kst[j].w[w];
-                        vw.w[w] = kConvert ? pack2<_Float16>(half_lo<T>(vst[j].w[w]),
-                                                             half_hi<T>(vst[j].w[w]))
-                                           : vst[j].w[w];
-                    }
-                    kw.w[w] = keep ? kw.w[w] : 0u;
-                    vw.w[w] = keep ? vw.w[w] : 0u;
+                for (int x = 0; x < PT; ++x) {
+                    const int d = 8 * (piece0 + LPR * x);
+                    to[j][x] = load_bytes<EBP>(base + off[j] + (d < D ? d : 0) * EB);
                 }
-                *reinterpret_cast<U16x8*>(kt + tok * K_LD + piece * 8) = kw;
-                *reinterpret_cast<U16x8*>(vt + tok * V_LD + piece * 8) = vw;
+        };
+        // Rows past the end and dims past the head's are zeros in LDS.
+        auto trim = [&](Bytes<EBP> (&to)[JT][PT], int i) {
+            const int left = k1 - k0 - i * BK;
+            if (left < BK || D < DP) {
+                asm volatile("");  // (rare: a branch, not selects)
+#pragma unroll
+                for (int j = 0; j < JT; ++j)
+#pragma unroll
+                    for (int x = 0; x < PT; ++x)
+                        if (tok0 + j * TSTEP >= left || 8 * (piece0 + LPR * x) >= D)
+                            to[j][x] = Bytes<EBP>{};
             }
+        };
+        auto store_k = [&](const Stage& st, int i) {
+            uint16_t* const kt = ks + (i & 1) * K_TILE;
+            if (TSTEP > BK && tok0 >= BK) return;
+#pragma unroll
+            for (int j = 0; j < JT; ++j)
+#pragma unroll
+                for (int x = 0; x < PT; ++x) {
+                    U16x8 w8;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        if constexpr (F8)
+                            w8.w[w] = (w & 1) ? widen2<T, true>(st.k[j][x].w[w >> 1])
+                                              : widen2<T, false>(st.k[j][x].w[w >> 1]);
+                        else
+                            w8.w[w] = st.k[j][x].w[w];
+                    }
+                    *reinterpret_cast<U16x8*>(kt + (tok0 + j * TSTEP) * K_LD +
+                                              8 * (piece0 + LPR * x)) = w8;
+                }
+        };
+        auto store_v = [&](const Stage& st, int i) {
+            uint16_t* const vt = vs + (i & 1) * V_TILE;
+            if (TSTEP > BK && tok0 >= BK) return;
+#pragma unroll
+            for (int j = 0; j < JT; ++j)
+#pragma unroll
+                for (int x = 0; x < PT; ++x) {
+                    U16x8 w8;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        if constexpr (F8)
+                            w8.w[w] = (w & 1) ? widen2<_Float16, true>(st.v[j][x].w[w >> 1])
+                                              : widen2<_Float16, false>(st.v[j][x].w[w >> 1]);
+                        else if constexpr (kConvert)
+                            w8.w[w] = pack2<_Float16>(half_lo<T>(st.v[j][x].w[w]),
+                                                      half_hi<T>(st.v[j][x].w[w]));
+                        else
+                            w8.w[w] = st.v[j][x].w[w];
+                    }
+                    *reinterpret_cast<U16x8*>(vt + (tok0 + j * TSTEP) * V_LD +
+                                              8 * (piece0 + LPR * x)) = w8;
+                }
         };
 
         f32x16 o[ND];  // O^T: lane = (dims 32n + 8g + 4*half + i, query col)
 #pragma unroll
         for (int n = 0; n < ND; ++n) o[n] = f32x16{};
         float m_run = -INFINITY, l_run = 0.f;
-
-        load_ids(0);
-        load_tile(0);
-        load_ids(1);
-        store_tile(0);
-        load_tile(1);
-        load_ids(2);
-        for (int i = 0; i < ntiles; ++i) {
-            // Tile i is in LDS, and nobody reads tile i - 1 any more.
-            __syncthreads();
-            store_tile(i + 1);
-            load_tile(i + 2);
-            load_ids(i + 3);
-            if (!active) continue;
-            const uint16_t* const kt = ks + (i & 1) * K_TILE;
-            const uint16_t* const vt = vs + (i & 1) * V_TILE;
-
-            f32x16 sc[TB];  // S^T: token 32tb + 8(v/4) + 4*half + v%4
-#pragma unroll
-            for (int tb = 0; tb < TB; ++tb) sc[tb] = f32x16{};
+        U16x8 pb[2] = {};  // weights of the last tile, not yet multiplied with its V:
+                           // step s's token 16s + 8jj + 4*half + i at k = 4jj + i
+        // S^T of a tile: token 8(v/4) + 4*half + v%4 of the lane's query.
+        auto scores = [&](int i, f32x16& sc) {
+            const uint16_t* const kt = ks + (i & 1) * K_TILE + col * K_LD + 8 * half;
+            sc = f32x16{};
 #pragma unroll
             for (int c = 0; c < NC; ++c)
+                sc = mfma_32x32x16<T>(*reinterpret_cast<const U16x8*>(kt + 16 * c), qv[c], sc);
+        };
+        const int vlane = (4 * half + ((lane & 15) >> 2)) * V_LD + 16 * ((lane >> 4) & 1) +
+                          4 * (lane & 3);
+        auto values = [&](int i) {  // O^T += V^T P^T of tile i, whose weights are in pb
+            const uint16_t* const vt = vs + (i & 1) * V_TILE + vlane;
 #pragma unroll
-                for (int tb = 0; tb < TB; ++tb) {
-                    const U16x8 kk = *reinterpret_cast<const U16x8*>(
-                        kt + (32 * tb + col) * K_LD + 16 * c + 8 * half);
-                    sc[tb] = mfma_32x32x16<T>(kk, qv[c], sc[tb]);
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int n = 0; n < ND; ++n) {
+                    const uint2 lo = read_transposed(vt + (16 * s) * V_LD + 32 * n);
+                    const uint2 hi = read_transposed(vt + (16 * s + 8) * V_LD + 32 * n);
+                    const U16x8 va = {{lo.x, lo.y, hi.x, hi.y}};
+                    o[n] = mfma_32x32x16<_Float16>(va, pb[s], o[n]);
                 }
+        };
+        // Step i. LDS holds K of two tiles and V of two: K of i + 1 is read while
+        // K of i + 2 is written (over i's), V of i - 1 read and V of i written
+        // (over i - 2's).
+        // Loads come back in order, so the ids go out ahead of the rows: the next
+        // step waits for them and not for rows.
+        auto stage = [&](Stage& st, int i) {
+            store_k(st, i + 2);
+            store_v(st, i);
+            uint64_t voff[JT];
+#pragma unroll
+            for (int j = 0; j < JT; ++j) voff[j] = st.off[j];  // tile i + 2's rows
+            locate(st, i + 4);
+            load_ids(i + 5);
+            load(st.v, voff, vbase);
+            load(st.k, st.off, kbase);
+        };
+        // The scores of the next tile, the weights of this one and the products
+        // of the last one have nothing to wait for in each other, so the matrix
+        // cores work while the vector units do.
+        auto step = [&](Stage& st, int i, f32x16& sc, f32x16& next) {
+            __syncthreads();
+            trim(st.k, i + 2);
+            trim(st.v, i);
             const int left = k1 - k0 - i * BK;
             if (left < BK) {
+                asm volatile("");  // a branch, not selects
 #pragma unroll
-                for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                        if (32 * tb + 8 * (v >> 2) + 4 * half + (v & 3) >= left)
-                            sc[tb][v] = -INFINITY;
+                for (int v = 0; v < 16; ++v)
+                    if (8 * (v >> 2) + 4 * half + (v & 3) >= left) sc[v] = -INFINITY;
             }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) mx[v & 3] = fmaxf(mx[v & 3], sc[tb][v]);
-            const float cm =
-                pair_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))) * a.scale_log2;
+            for (int v = 0; v < 16; ++v) mx[v & 1] = fmaxf(mx[v & 1], sc[v]);
+            const float cm = pair_max(fmaxf(mx[0], mx[1])) * a.scale_log2;
             const bool grow = cm > m_run + kSlack;  // also: first finite maximum
-            float alpha = 1.f;
-            if (grow) {
-                alpha = __builtin_amdgcn_exp2f(m_run - cm);
-                m_run = cm;
-            }
             if (__builtin_amdgcn_ballot_w64(grow)) {
+                values(i - 1);  // at the old maximum
+                pb[0] = pb[1] = U16x8{};
+                const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - cm) : 1.f;
+                m_run = grow ? cm : m_run;
                 l_run *= alpha;
 #pragma unroll
                 for (int n = 0; n < ND; ++n) o[n] *= alpha;
             }
+            scores(i + 1, next);
+            U16x8 pn[2];
             const float m_use = m_run == -INFINITY ? 0.f : m_run - kShift;
-            U16x8 pb[2 * TB];  // P, step st: token 16st + 8jj + 4*half + i at k = 4jj + i
-            float ps[4] = {0.f, 0.f, 0.f, 0.f};
+            float ps[2] = {0.f, 0.f};
 #pragma unroll
-            for (int tb = 0; tb < TB; ++tb)
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int sh = 0; sh < 2; ++sh)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float p0 = __builtin_amdgcn_exp2f(
-                            __builtin_fmaf(sc[tb][8 * sh + 2 * e], a.scale_log2, -m_use));
-                        const float p1 = __builtin_amdgcn_exp2f(
-                            __builtin_fmaf(sc[tb][8 * sh + 2 * e + 1], a.scale_log2, -m_use));
-                        const uint32_t hw = pack2<_Float16>(p0, p1);
-                        pb[2 * tb + sh].w[e] = hw;
-                        // The denominator sums the fp16 weights that P.V uses.
-                        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-                        const h2 ones = {1.f16, 1.f16};
-                        ps[e] = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, hw), ones, ps[e],
-                                                       false);
-                    }
-            l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-            const int sub = (lane >> 4) & 1;  // which 16 dims this lane's block reads
-            const uint16_t* const vl =
-                vt + (4 * half + ((lane & 15) >> 2)) * V_LD + 16 * sub + 4 * (lane & 3);
-#pragma unroll
-            for (int st = 0; st < 2 * TB; ++st)
-#pragma unroll
-                for (int n = 0; n < ND; ++n) {
-                    const uint2 lo = read_transposed(vl + (16 * st) * V_LD + 32 * n);
-                    const uint2 hi = read_transposed(vl + (16 * st + 8) * V_LD + 32 * n);
-                    const U16x8 va = {{lo.x, lo.y, hi.x, hi.y}};
-                    o[n] = mfma_32x32x16<_Float16>(va, pb[st], o[n]);
+                for (int e = 0; e < 4; ++e) {
+                    const float p0 = __builtin_amdgcn_exp2f(
+                        __builtin_fmaf(sc[8 * s + 2 * e], a.scale_log2, -m_use));
+                    const float p1 = __builtin_amdgcn_exp2f(
+                        __builtin_fmaf(sc[8 * s + 2 * e + 1], a.scale_log2, -m_use));
+                    const uint32_t hw = pack2<_Float16>(p0, p1);
+                    pn[s].w[e] = hw;
+                    // The denominator sums the fp16 weights that P.V uses.
+                    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+                    const h2 ones = {1.f16, 1.f16};
+                    ps[s] = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, hw), ones, ps[s], false);
                 }
+            l_run += ps[0] + ps[1];
+            values(i - 1);
+            stage(st, i);
+            pb[0] = pn[0];
+            pb[1] = pn[1];
+            interleave<NC, ND>();
+        };
+
+        // The loads stay in this order (the loop's waits count on what is behind
+        // a load on every way in).
+        f32x16 sa, sb;
+        auto keep_order = []() { __builtin_amdgcn_sched_barrier(0); };
+        load_ids(0);
+        locate(st0, 0);
+        load_ids(1);
+        keep_order();
+        load(st0.k, st0.off, kbase);
+        load(st0.v, st0.off, vbase);
+        keep_order();
+        locate(st1, 1);
+        load_ids(2);
+        keep_order();
+        load(st1.k, st1.off, kbase);
+        load(st1.v, st1.off, vbase);
+        keep_order();
+        trim(st0.k, 0);
+        store_k(st0, 0);
+        locate(st0, 2);
+        load_ids(3);
+        keep_order();
+        load(st0.k, st0.off, kbase);
+        keep_order();
+        trim(st1.k, 1);
+        store_k(st1, 1);
+        store_v(st1, 1);  // step 0 multiplies these with weights of 0: numbers, at least
+        locate(st1, 3);
+        load_ids(4);
+        keep_order();
+        load(st1.k, st1.off, kbase);
+        keep_order();
+        __syncthreads();
+        scores(0, sa);
+        // Two steps a round, the second past the end where the tiles are odd in
+        // number (its weights are 0): a way around it would lead the loop's
+        // waits to expect the first one's loads at once.
+        const int steps = (ntiles + 1) & ~1;
+        for (int i = 0; i < steps; i += 2) {
+            step(st0, i, sa, sb);
+            step(st1, i + 1, sb, sa);
         }
+        __syncthreads();  // V of the last tile
+        values(steps - 1);
 
         bool again = false;
         if constexpr (kConvert) {
@@ -496,6 +614,11 @@ shared_prefix_tasks(Args<T> a) {
         constexpr int E = DP / 16;             // V elements per lane and token
         constexpr int VL = DP == 256 ? 2 : 1;  // loads that hold them
         constexpr int VB = E * EB / VL;        // bytes of one
+        // A thread id of its own: nothing derived from it is worked out ahead of
+        // the wide path, whose registers it would take.
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
         const int col = lane & 15, quad = lane >> 4;
         f32x4 acc[E];  // query 4*quad + v, this lane's dim e
 #pragma unroll
@@ -587,12 +710,17 @@ shared_prefix_tasks(Args<T> a) {
                         d = mfma32<T>(kk, qb[c], d);
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int t = t0 + 16 * j + 4 * quad + i;
-                        s[j][i] = t < t_end ? d[i] * a.scale_log2 : -INFINITY;
-                    }
+                    for (int i = 0; i < 4; ++i) s[j][i] = d[i] * a.scale_log2;
                 }
                 load_k(next);
+                if (t0 + CH > t_end) {
+                    asm volatile("");  // a branch, not selects
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (t0 + 16 * j + 4 * quad + i >= t_end) s[j][i] = -INFINITY;
+                }
 
                 float cmax = -INFINITY;
 #pragma unroll
@@ -624,6 +752,7 @@ shared_prefix_tasks(Args<T> a) {
                 // Rows past the end hold the last token again: their weight is
                 // 0, but 0 * inf is not.
                 if (t0 + CH > t_end) {
+                    asm volatile("");
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -734,40 +863,74 @@ shared_prefix_tasks(Args<T> a) {
 }
 
 // out = v_scale * sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the parts
-// of a (row, head), DP / 4 lanes each; rows without keys are zeros, rows of one
-// part are already written.
+// of a (row, head); rows without keys are zeros, rows of one part are already
+// written. A wave each: DP / 4 lanes hold a part's dims, so 64 / (DP / 4)
+// parts load at once, eight rounds of them ahead of their use, and lane s
+// holds the (max, sum) of part s.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads)
 shared_prefix_merge(Args<T> a) {
-    constexpr int LPH = DP / 4;
+    constexpr int LPH = DP / 4, PAR = 64 / LPH, B = 8;
     const int32_t* const plan = a.plan;
     if (plan[H_ROWS] != a.num_rows || plan[H_HEADS] != a.heads || plan[H_DIM] != a.head_dim ||
         plan[H_PARTS] > a.entries)
         return;
-    const int64_t item = (int64_t(blockIdx.x) * kThreads + threadIdx.x) / LPH;
+    const int64_t item = int64_t(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
     if (item >= int64_t(a.num_rows) * a.heads) return;
     const int r = int(item / a.heads), h = int(item - int64_t(r) * a.heads);
-    const int d = 4 * int(threadIdx.x % LPH);
+    const int lane = threadIdx.x & 63, sub = lane / LPH, d = 4 * (lane % LPH);
     const int parts = plan[a.rows_at + 2 * r + 1];
-    if (d >= a.head_dim || parts == 1) return;
+    if (parts == 1) return;
+    const bool has = d < a.head_dim;
     const int64_t first = int64_t(plan[a.rows_at + 2 * r]) * a.heads + h;
+    const float2* const pml = a.part_ml + first;
+    const float* const po = a.part_o + first * a.head_dim + (has ? d : 0);
+    const int64_t step = int64_t(a.heads) * a.head_dim;
+    auto load = [&](int s0, float4 (&o)[B]) {  // past the last part: that again, at weight 0
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+            o[i] = *reinterpret_cast<const float4*>(po +
+                                                    min(s0 + i * PAR + sub, parts - 1) * step);
+    };
+    float4 o[B];
+    if (parts) load(0, o);
     float mx = -INFINITY;
-    for (int s = 0; s < parts; ++s) mx = fmaxf(mx, a.part_ml[first + int64_t(s) * a.heads].x);
+    for (int s0 = 0; s0 < parts; s0 += 64)
+        if (s0 + lane < parts) mx = fmaxf(mx, pml[int64_t(s0 + lane) * a.heads].x);
+    mx = wave_max(mx);
     const float m_use = mx == -INFINITY ? 0.f : mx;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < parts; ++s) {
-        const int64_t e = first + int64_t(s) * a.heads;
-        const float2 ml = a.part_ml[e];
-        const float4 p = *reinterpret_cast<const float4*>(a.part_o + e * a.head_dim + d);
-        const float f = __builtin_amdgcn_exp2f(ml.x - m_use);
-        l += f * ml.y;
-        sum.x += f * p.x;
-        sum.y += f * p.y;
-        sum.z += f * p.z;
-        sum.w += f * p.w;
+    for (int s0 = 0; s0 < parts; s0 += 64) {
+        float w = 0.f;
+        if (s0 + lane < parts) {
+            const float2 ml = pml[int64_t(s0 + lane) * a.heads];
+            w = __builtin_amdgcn_exp2f(ml.x - m_use);
+            l += w * ml.y;
+        }
+        for (int s1 = s0; s1 < min(s0 + 64, parts); s1 += B * PAR) {
+            if (s1 > 0) load(s1, o);
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                const int s = s1 + i * PAR + sub;
+                float f = __shfl(w, (s - s0) & 63, 64);
+                f = s < min(s0 + 64, parts) ? f : 0.f;
+                sum.x += f * o[i].x;
+                sum.y += f * o[i].y;
+                sum.z += f * o[i].z;
+                sum.w += f * o[i].w;
+            }
+        }
     }
+    l = wave_sum(l);
+#pragma unroll
+    for (int off = LPH; off < 64; off <<= 1) {
+        sum.x += __shfl_xor(sum.x, off, 64);
+        sum.y += __shfl_xor(sum.y, off, 64);
+        sum.z += __shfl_xor(sum.z, off, 64);
+        sum.w += __shfl_xor(sum.w, off, 64);
+    }
+    if (sub != 0 || !has) return;
     const float inv = parts == 0 ? 0.f : a.v_scale / l;
     uint2 w;
     w.x = pack2<T>(sum.x * inv, sum.y * inv);
@@ -1046,8 +1209,8 @@ extern "C" int tvllm_paged_decode_shared_prefix(
         // (t m) >> (31 + s) is t / d for every t < 2^31.
         int sh = 0;
         while ((int64_t(1) << sh) < block_size) ++sh;
-        a.page_shift = 31 + sh;
-        a.page_mul = uint32_t(((uint64_t(1) << a.page_shift) + uint64_t(block_size) - 1) /
+        a.page_shift = sh;
+        a.page_mul = uint32_t(((uint64_t(1) << (31 + sh)) + uint64_t(block_size) - 1) /
                               uint64_t(block_size));
         a.scale_log2 = scale * kLog2e * k_scale;
         a.v_scale = v_scale;
@@ -1059,9 +1222,8 @@ extern "C" int tvllm_paged_decode_shared_prefix(
                 if (f8) shared_prefix_tasks<T, DP, true><<<int(num_tasks), kThreads, 0, s>>>(a);
                 else shared_prefix_tasks<T, DP, false><<<int(num_tasks), kThreads, 0, s>>>(a);
             }
-            const int64_t threads = num_rows * num_heads * (DP / 4);
             shared_prefix_merge<T, DP>
-                <<<int((threads + kThreads - 1) / kThreads), kThreads, 0, s>>>(a);
+                <<<int(div_up(num_rows * num_heads, kThreads / 64)), kThreads, 0, s>>>(a);
         };
         if (head_dim <= 32) go.template operator()<32>();
         else if (head_dim <= 64) go.template operator()<64>();

@@ -59,8 +59,8 @@ constexpr int kTaskWords = 8;
 enum Header { H_TASKS, H_ROWS, H_HEADS, H_KV_HEADS, H_DIM, H_BLOCK, H_PARTS };
 // A task's queries are number q_begin .. + q_count - 1 of its group's, query i
 // being head i % group (of the KV head) of row members[member + i / group]; its
-// keys are tokens k0 .. k1 - 1 of the first such row's table.
-enum Task { T_MEMBER, T_QBEGIN, T_QCOUNT, T_KVH, T_K0, T_K1, T_PART, T_UNUSED };
+// keys are tokens k0 .. k1 - 1 of the table of row T_ROW, the first of them.
+enum Task { T_MEMBER, T_QBEGIN, T_QCOUNT, T_KVH, T_K0, T_K1, T_PART, T_ROW };
 
 constexpr int64_t kTargetTasks = 512;  // two workgroups per CU
 constexpr int64_t kKeyUnit = 64;       // tasks' key ranges are multiples of this
@@ -266,7 +266,7 @@ shared_prefix_tasks(Args<T> a) {
     const int k0 = task[T_K0], k1 = task[T_K1], part = task[T_PART];
     const int D = a.head_dim;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int64_t table = a.offsets[members[q_begin / a.group]];
+    const int64_t table = a.offsets[task[T_ROW]];
     const uint32_t* const ids = reinterpret_cast<const uint32_t*>(a.blocks + table);
     const uint32_t row_bytes = uint32_t(a.css * EB);
     const char* const kbase = static_cast<const char*>(a.k) + int64_t(kvh) * a.chs * EB;
@@ -340,15 +340,15 @@ shared_prefix_tasks(Args<T> a) {
         auto token_of = [&](int i, int j) {  // past the end: the last token again
             return min(uint32_t(k0 + i * BK + tok0 + j * TSTEP), last);
         };
-        auto load_ids = [&](int i) {
+        auto load_ids = [&](uint32_t (&id)[JT], int i) {
 #pragma unroll
             for (int j = 0; j < JT; ++j) id[j] = ids[2 * uint64_t(page_of(token_of(i, j)))];
         };
-        auto locate = [&](Stage& st, int i) {  // tile i's rows, by the ids loaded for it
+        auto locate = [&](uint64_t (&off)[JT], const uint32_t (&id)[JT], int i) {  // tile i's rows
 #pragma unroll
             for (int j = 0; j < JT; ++j) {
                 const uint32_t t = token_of(i, j);
-                st.off[j] = uint64_t(slot_of(id[j], t, page_of(t))) * row_bytes;
+                off[j] = uint64_t(slot_of(id[j], t, page_of(t))) * row_bytes;
             }
         };
         auto load = [&](Bytes<EBP> (&to)[JT][PT], const uint64_t (&off)[JT], const char* base) {
@@ -373,7 +373,7 @@ shared_prefix_tasks(Args<T> a) {
                             to[j][x] = Bytes<EBP>{};
             }
         };
-        auto store_k = [&](const Stage& st, int i) {
+        auto store_k = [&](const Bytes<EBP> (&k)[JT][PT], int i) {
             uint16_t* const kt = ks + (i & 1) * K_TILE;
             if (TSTEP > BK && tok0 >= BK) return;
 #pragma unroll
@@ -384,16 +384,16 @@ shared_prefix_tasks(Args<T> a) {
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         if constexpr (F8)
-                            w8.w[w] = (w & 1) ? widen2<T, true>(st.k[j][x].w[w >> 1])
-                                              : widen2<T, false>(st.k[j][x].w[w >> 1]);
+                            w8.w[w] = (w & 1) ? widen2<T, true>(k[j][x].w[w >> 1])
+                                              : widen2<T, false>(k[j][x].w[w >> 1]);
                         else
-                            w8.w[w] = st.k[j][x].w[w];
+                            w8.w[w] = k[j][x].w[w];
                     }
                     *reinterpret_cast<U16x8*>(kt + (tok0 + j * TSTEP) * K_LD +
                                               8 * (piece0 + LPR * x)) = w8;
                 }
         };
-        auto store_v = [&](const Stage& st, int i) {
+        auto store_v = [&](const Bytes<EBP> (&v)[JT][PT], int i) {
             uint16_t* const vt = vs + (i & 1) * V_TILE;
             if (TSTEP > BK && tok0 >= BK) return;
 #pragma unroll
@@ -404,13 +404,13 @@ shared_prefix_tasks(Args<T> a) {
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         if constexpr (F8)
-                            w8.w[w] = (w & 1) ? widen2<_Float16, true>(st.v[j][x].w[w >> 1])
-                                              : widen2<_Float16, false>(st.v[j][x].w[w >> 1]);
+                            w8.w[w] = (w & 1) ? widen2<_Float16, true>(v[j][x].w[w >> 1])
+                                              : widen2<_Float16, false>(v[j][x].w[w >> 1]);
                         else if constexpr (kConvert)
-                            w8.w[w] = pack2<_Float16>(half_lo<T>(st.v[j][x].w[w]),
-                                                      half_hi<T>(st.v[j][x].w[w]));
+                            w8.w[w] = pack2<_Float16>(half_lo<T>(v[j][x].w[w]),
+                                                      half_hi<T>(v[j][x].w[w]));
                         else
-                            w8.w[w] = st.v[j][x].w[w];
+                            w8.w[w] = v[j][x].w[w];
                     }
                     *reinterpret_cast<U16x8*>(vt + (tok0 + j * TSTEP) * V_LD +
                                               8 * (piece0 + LPR * x)) = w8;
@@ -451,13 +451,13 @@ shared_prefix_tasks(Args<T> a) {
         // Loads come back in order, so the ids go out ahead of the rows: the next
         // step waits for them and not for rows.
         auto stage = [&](Stage& st, int i) {
-            store_k(st, i + 2);
-            store_v(st, i);
+            store_k(st.k, i + 2);
+            store_v(st.v, i);
             uint64_t voff[JT];
 #pragma unroll
             for (int j = 0; j < JT; ++j) voff[j] = st.off[j];  // tile i + 2's rows
-            locate(st, i + 4);
-            load_ids(i + 5);
+            locate(st.off, id, i + 4);
+            load_ids(id, i + 5);
             load(st.v, voff, vbase);
             load(st.k, st.off, kbase);
         };
@@ -516,38 +516,43 @@ shared_prefix_tasks(Args<T> a) {
             interleave<NC, ND>();
         };
 
-        // The loads stay in this order (the loop's waits count on what is behind
-        // a load on every way in).
+        // Everything the first steps need goes out before anything is waited for,
+        // in the order in which it is needed (the loop's waits count on what is
+        // behind a load on every way in).
         f32x16 sa, sb;
-        auto keep_order = []() { __builtin_amdgcn_sched_barrier(0); };
-        load_ids(0);
-        locate(st0, 0);
-        load_ids(1);
-        keep_order();
-        load(st0.k, st0.off, kbase);
-        load(st0.v, st0.off, vbase);
-        keep_order();
-        locate(st1, 1);
-        load_ids(2);
-        keep_order();
-        load(st1.k, st1.off, kbase);
-        load(st1.v, st1.off, vbase);
-        keep_order();
-        trim(st0.k, 0);
-        store_k(st0, 0);
-        locate(st0, 2);
-        load_ids(3);
-        keep_order();
-        load(st0.k, st0.off, kbase);
-        keep_order();
-        trim(st1.k, 1);
-        store_k(st1, 1);
-        store_v(st1, 1);  // step 0 multiplies these with weights of 0: numbers, at least
-        locate(st1, 3);
-        load_ids(4);
-        keep_order();
-        load(st1.k, st1.off, kbase);
-        keep_order();
+        {
+            auto keep_order = []() { __builtin_amdgcn_sched_barrier(0); };
+            uint32_t id0[JT], id1[JT], id2[JT], id3[JT];
+            uint64_t off0[JT], off1[JT];
+            Bytes<EBP> first[JT][PT], second[JT][PT];
+            load_ids(id0, 0);
+            load_ids(id1, 1);
+            load_ids(id2, 2);
+            load_ids(id3, 3);
+            load_ids(id, 4);
+            locate(off0, id0, 0);
+            locate(off1, id1, 1);
+            locate(st0.off, id2, 2);
+            locate(st1.off, id3, 3);
+            keep_order();
+            load(first, off0, kbase);
+            load(second, off1, kbase);
+            keep_order();
+            load(st0.v, off0, vbase);
+            load(st0.k, st0.off, kbase);
+            keep_order();
+            load(st1.v, off1, vbase);
+            load(st1.k, st1.off, kbase);
+            keep_order();
+            // Step 0 multiplies what stands in place of tile -1's V with weights
+            // of 0: zeros, as LDS may hold NaNs.
+            for (int x = tid; x < V_TILE / 8; x += kThreads)
+                reinterpret_cast<U16x8*>(vs + V_TILE)[x] = U16x8{};
+            trim(first, 0);
+            store_k(first, 0);
+            trim(second, 1);
+            store_k(second, 1);
+        }
         __syncthreads();
         scores(0, sa);
         // Two steps a round, the second past the end where the tiles are odd in
@@ -558,6 +563,8 @@ shared_prefix_tasks(Args<T> a) {
             step(st0, i, sa, sb);
             step(st1, i + 1, sb, sa);
         }
+        bool direct;
+        const int64_t entry = entry_of(row, head, direct);
         __syncthreads();  // V of the last tile
         values(steps - 1);
 
@@ -574,8 +581,6 @@ shared_prefix_tasks(Args<T> a) {
         if (__syncthreads_or(again)) return true;
         const float l = pair_sum(l_run);
         if (qi >= q_count) return false;
-        bool direct;
-        const int64_t entry = entry_of(row, head, direct);
         if (direct) {
             const float inv = a.v_scale / l;
             T* orow = a.out + a.rows[row] * a.ots + head * a.ohs + 4 * half;
@@ -669,6 +674,7 @@ shared_prefix_tasks(Args<T> a) {
             };
 
             uint32_t id = load_id(t_begin);
+            uint32_t id2 = load_id(t_begin + CH);
             U16x8 qb[KS];  // B operand: query col, dims 32c + 8*quad ..
             {
                 int row, head;
@@ -682,7 +688,7 @@ shared_prefix_tasks(Args<T> a) {
             }
             {
                 const uint32_t slot = resolve(t_begin, id);
-                id = load_id(t_begin + CH);
+                id = id2;
                 load_k(slot);
                 load_v(slot);
             }
@@ -1049,7 +1055,7 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
             t[T_K0] = int32_t(k0);
             t[T_K1] = int32_t(k1);
             t[T_PART] = int32_t(part);
-            t[T_UNUSED] = 0;
+            t[T_ROW] = members[member + q0 / group];
         };
         // Shared keys first, the longest tasks ahead. Workgroups are dealt to
         // the 8 XCDs in turn: the query tiles of one (KV head, range of keys)

@@ -62,10 +62,13 @@ enum Header { H_TASKS, H_ROWS, H_HEADS, H_KV_HEADS, H_DIM, H_BLOCK, H_PARTS };
 // keys are tokens k0 .. k1 - 1 of the table of row T_ROW, the first of them.
 enum Task { T_MEMBER, T_QBEGIN, T_QCOUNT, T_KVH, T_K0, T_K1, T_PART, T_ROW };
 
-constexpr int64_t kTargetTasks = 512;  // two workgroups per CU
-constexpr int64_t kKeyUnit = 64;       // tasks' key ranges are multiples of this
-constexpr int64_t kMinKeys = 256;      // no split makes shorter tasks
-constexpr int64_t kMaxParts = 64;      // splits of one unit
+constexpr int64_t kSlots = 512;     // workgroups at once: two on each of 256 CUs
+constexpr int64_t kKeyUnit = 64;    // tasks' key ranges are multiples of this
+constexpr int64_t kMaxParts = 64;   // splits of one unit
+constexpr int64_t kMaxSplits = 1024;  // tasks that splitting adds, all units together
+// What a task costs beside its keys (its chain of first loads, the merge in LDS
+// and the write of its part), in keys.
+constexpr int64_t kTaskCost = 128;
 
 struct PlanLayout {
     int64_t rows_at, members_at, tasks_at, max_tasks, words;
@@ -75,10 +78,10 @@ PlanLayout plan_layout(int64_t max_rows, int64_t heads, int64_t kv_heads) {
     const int64_t group = heads / kv_heads;
     PlanLayout p;
     // Every unit (KV head, tile of queries) of keys K makes at most K / chunk
-    // + 1 tasks, and chunk >= all units' keys / kTargetTasks.
+    // + 1 tasks, and chunk >= all units' keys / kMaxSplits.
     const int64_t own = max_rows * ((group + kWide - 1) / kWide);
     const int64_t shared = (max_rows * group + kWide - 1) / kWide + max_rows / 2;
-    p.max_tasks = kTargetTasks + kv_heads * (own + shared);
+    p.max_tasks = kMaxSplits + kv_heads * (own + shared);
     p.rows_at = kHeader;
     p.members_at = p.rows_at + 2 * max_rows;
     p.tasks_at = p.members_at + max_rows;
@@ -89,7 +92,7 @@ PlanLayout plan_layout(int64_t max_rows, int64_t heads, int64_t kv_heads) {
 // (row part, query head) results of one call at most: a unit of q queries and
 // K keys makes q (K / chunk + 1) of them.
 int64_t max_entries(int64_t max_rows, int64_t heads) {
-    return 2 * max_rows * heads + kWide * kTargetTasks;
+    return 2 * max_rows * heads + kWide * kMaxSplits;
 }
 
 // ---------------------------------------------------------------- device --
@@ -179,18 +182,35 @@ __device__ __forceinline__ float pair_sum(float x) {
     return as_f(r[0]) + as_f(r[1]);
 }
 
-// N bytes from memory as they lie there; rows read once go past the caches.
+// N bytes from memory as they lie there. STREAM: lines that an instruction takes
+// whole and nobody else reads go past the caches (V of the narrow path; where an
+// instruction takes half a line of each row, the other half would be fetched
+// again: own keys of 256 rows x 2048, 375 us with K through the caches, 401 past
+// them).
 template <int N>
 struct Bytes {
     uint32_t w[(N + 3) / 4];
 };
 
-template <int N>
+template <int N, bool STREAM>
 __device__ __forceinline__ Bytes<N> load_bytes(const char* p) {
     typedef uint32_t u2 __attribute__((ext_vector_type(2)));
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
     Bytes<N> r;
-    if constexpr (N == 2) {
+    if constexpr (!STREAM) {
+        if constexpr (N == 16) {
+            const u4 t = *reinterpret_cast<const u4*>(p);
+            r.w[0] = t[0];
+            r.w[1] = t[1];
+            r.w[2] = t[2];
+            r.w[3] = t[3];
+        } else {
+            static_assert(N == 8);
+            const u2 t = *reinterpret_cast<const u2*>(p);
+            r.w[0] = t[0];
+            r.w[1] = t[1];
+        }
+    } else if constexpr (N == 2) {
         r.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(p));
     } else if constexpr (N == 4) {
         r.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
@@ -357,7 +377,7 @@ shared_prefix_tasks(Args<T> a) {
 #pragma unroll
                 for (int x = 0; x < PT; ++x) {
                     const int d = 8 * (piece0 + LPR * x);
-                    to[j][x] = load_bytes<EBP>(base + off[j] + (d < D ? d : 0) * EB);
+                    to[j][x] = load_bytes<EBP, false>(base + off[j] + (d < D ? d : 0) * EB);
                 }
         };
         // Rows past the end and dims past the head's are zeros in LDS.
@@ -479,8 +499,10 @@ shared_prefix_tasks(Args<T> a) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) mx[v & 1] = fmaxf(mx[v & 1], sc[v]);
             const float cm = pair_max(fmaxf(mx[0], mx[1])) * a.scale_log2;
-            const bool grow = cm > m_run + kSlack;  // also: first finite maximum
-            if (__builtin_amdgcn_ballot_w64(grow)) {
+            const bool grow = cm > m_run + kSlack;  // also: a first finite maximum
+            if (i == 0) {  // (nothing to rescale yet)
+                m_run = cm;
+            } else if (__builtin_amdgcn_ballot_w64(grow)) {
                 values(i - 1);  // at the old maximum
                 pb[0] = pb[1] = U16x8{};
                 const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - cm) : 1.f;
@@ -613,7 +635,8 @@ shared_prefix_tasks(Args<T> a) {
     // ----------------------------------------------------------- narrow --
     // Queries q0 .. q0 + qn - 1 (qn <= 16) of the task over its keys.
     auto narrow = [&](int q0, int qn) {
-        constexpr int NT = DP == 256 ? 1 : DP == 128 ? 2 : 4;  // 16-token tiles per chunk
+        // 16-token tiles per chunk: 16 KB of K and V in flight per wave
+        constexpr int NT = DP == 256 ? 1 : DP == 128 ? (F8 ? 4 : 2) : 4;
         constexpr int CH = 16 * NT;
         constexpr int KS = DP / 32;            // k-steps of Q.K^T
         constexpr int E = DP / 16;             // V elements per lane and token
@@ -654,7 +677,7 @@ shared_prefix_tasks(Args<T> a) {
 #pragma unroll
                     for (int c = 0; c < KS; ++c) {
                         const int d = 32 * c + 8 * quad;
-                        kreg[j][c] = load_bytes<8 * EB>(p + (d < D ? d : 0) * EB);
+                        kreg[j][c] = load_bytes<8 * EB, false>(p + (d < D ? d : 0) * EB);
                     }
                 }
             };
@@ -668,7 +691,7 @@ shared_prefix_tasks(Args<T> a) {
 #pragma unroll
                         for (int x = 0; x < VL; ++x) {
                             const int d = dim_of(x);
-                            vreg[j][i][x] = load_bytes<VB>(p + (d < D ? d : 0) * EB);
+                            vreg[j][i][x] = load_bytes<VB, true>(p + (d < D ? d : 0) * EB);
                         }
                     }
             };
@@ -1037,13 +1060,47 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
             cost += own_tiles * num_kv_heads * own[r];
         }
         for (const Group& g : gs) cost += div_up(g.count * group, kWide) * num_kv_heads * g.prefix;
-        const int64_t chunk =
-            std::max(kMinKeys, div_up(div_up(cost, kTargetTasks), kKeyUnit) * kKeyUnit);
-        auto cut = [&](int64_t keys, int64_t& splits, int64_t& per) {
+        auto cut = [](int64_t keys, int64_t chunk, int64_t& splits, int64_t& per) {
             splits = std::min(kMaxParts, div_up(keys, chunk));
             per = splits ? div_up(div_up(keys, splits), kKeyUnit) * kKeyUnit : 0;
             if (per) splits = div_up(keys, per);
         };
+        // The length of a task: the one that ends soonest by a simple estimate.
+        // Tasks run on kSlots slots, longest first: all at once where they are
+        // that few, otherwise the slots' mean share and half of a last, short
+        // task; and the parts are written and read again, an entry of 128 dims
+        // in about the time of 4 keys of a slot (8 bytes a dim, 512 bytes a key).
+        const int64_t least = std::max(kKeyUnit, div_up(cost, kMaxSplits));
+        int64_t chunk = 0;
+        double best = 0;
+        for (int64_t c = div_up(least, kKeyUnit) * kKeyUnit;; c += div_up(c, 4 * kKeyUnit) * kKeyUnit) {
+            int64_t count = 0, sum = 0, longest = 0, shortest = INT64_MAX, entries = 0, most = 0;
+            int64_t splits, per;
+            auto add = [&](int64_t units, int64_t queries, int64_t keys) {
+                cut(keys, c, splits, per);
+                count += units * splits;
+                sum += units * (keys + splits * kTaskCost);
+                longest = std::max(longest, std::min(per, keys) + kTaskCost);
+                shortest = std::min(shortest, std::min(per, keys) + kTaskCost);
+                entries += queries * splits;
+                most = std::max(most, keys);
+            };
+            for (const Group& g : gs)
+                if (g.prefix)
+                    add(div_up(g.count * group, kWide) * num_kv_heads, g.count * num_heads, g.prefix);
+            for (int64_t r = 0; r < num_rows; ++r)
+                if (own[r]) add(own_tiles * num_kv_heads, num_heads, own[r]);
+            const double time =
+                (count <= kSlots ? double(longest)
+                                 : std::max(double(longest), double(sum) / kSlots +
+                                                                 0.5 * double(shortest))) +
+                double(entries) * double(head_dim) / 32 / kSlots;
+            if (!chunk || time < best) {
+                chunk = c;
+                best = time;
+            }
+            if (c >= most) break;
+        }
         int64_t n = 0;
         auto emit = [&](int64_t member, int64_t q0, int64_t count, int64_t kvh, int64_t k0,
                         int64_t k1, int64_t part) {
@@ -1065,7 +1122,7 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
         };
         std::vector<int64_t> order;
         for (int64_t g = 0; g < num_groups; ++g) {
-            cut(gs[g].prefix, gs[g].splits, gs[g].per);
+            cut(gs[g].prefix, chunk, gs[g].splits, gs[g].per);
             if (gs[g].splits) order.push_back(g);
         }
         std::sort(order.begin(), order.end(), [&](int64_t x, int64_t y) {
@@ -1098,7 +1155,7 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
             const int64_t g = groups[r], shared = g >= 0 ? gs[g].splits : 0;
             const int64_t begin = g >= 0 ? gs[g].prefix : 0;
             int64_t splits, per;
-            cut(own[r], splits, per);
+            cut(own[r], chunk, splits, per);
             parts[r] = shared + splits;
             for (int64_t s = 0; s < splits; ++s)
                 for (int64_t t = 0; t < own_tiles; ++t)

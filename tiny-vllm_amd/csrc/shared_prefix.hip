@@ -57,10 +57,13 @@ constexpr float kShift = 7.f;
 constexpr int kHeader = 16;
 constexpr int kTaskWords = 8;
 enum Header { H_TASKS, H_ROWS, H_HEADS, H_KV_HEADS, H_DIM, H_BLOCK, H_PARTS };
-// A task's queries are number q_begin .. + q_count - 1 of its group's, query i
+// A task's queries are number q_begin .. + q_count - 1 of its group's (T_QUERIES:
+// q_begin / 16 above, q_count in the lower 8 bits), query i
 // being head i % group (of the KV head) of row members[member + i / group]; its
 // keys are tokens k0 .. k1 - 1 of the table of row T_ROW, the first of them.
-enum Task { T_MEMBER, T_QBEGIN, T_QCOUNT, T_KVH, T_K0, T_K1, T_PART, T_ROW };
+// T_HEADS (1, 2 or 4; above 1 in narrow tasks only): that many KV heads from T_KVH
+// on, each with its queries and keys.
+enum Task { T_MEMBER, T_QUERIES, T_KVH, T_HEADS, T_K0, T_K1, T_PART, T_ROW };
 
 constexpr int64_t kSlots = 512;     // workgroups at once: two on each of 256 CUs
 constexpr int64_t kKeyUnit = 64;    // tasks' key ranges are multiples of this
@@ -282,7 +285,8 @@ shared_prefix_tasks(Args<T> a) {
         return;
     const int32_t* const task = plan + a.tasks_at + int64_t(blockIdx.x) * kTaskWords;
     const int32_t* const members = plan + a.members_at + task[T_MEMBER];
-    const int q_begin = task[T_QBEGIN], q_count = task[T_QCOUNT], kvh = task[T_KVH];
+    const int q_begin = (task[T_QUERIES] >> 8) * kNarrow, q_count = task[T_QUERIES] & 0xff;
+    const int kvh = task[T_KVH];
     const int k0 = task[T_K0], k1 = task[T_K1], part = task[T_PART];
     const int D = a.head_dim;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -296,11 +300,11 @@ shared_prefix_tasks(Args<T> a) {
     auto slot_of = [&](uint32_t id, uint32_t t, uint32_t page) {
         return id * uint32_t(a.block_size) + (t - page * uint32_t(a.block_size));
     };
-    // Query i of the task: its row, and its head.
-    auto query = [&](int i, int& row, int& head) {
+    // Query i of the task, of KV head kvh + x: its row, and its head.
+    auto query = [&](int i, int x, int& row, int& head) {
         const int g = (q_begin + i) / a.group;
         row = members[g];
-        head = kvh * a.group + (q_begin + i - g * a.group);
+        head = (kvh + x) * a.group + (q_begin + i - g * a.group);
     };
     // Where a row's part goes; rows of one part are written to the output.
     auto entry_of = [&](int row, int head, bool& direct) -> int64_t {
@@ -328,7 +332,7 @@ shared_prefix_tasks(Args<T> a) {
         // the loop for them would make the others wait for its loads.
         const int qi = wave * 32 + col;
         int row, head;
-        query(min(qi, q_count - 1), row, head);
+        query(min(qi, q_count - 1), 0, row, head);
 
         U16x8 qv[NC];
         {
@@ -653,8 +657,13 @@ shared_prefix_tasks(Args<T> a) {
         for (int e = 0; e < E; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
         float m_run = -INFINITY, l_run = 0.f;
 
-        const int per = ((k1 - k0 + 3) / 4 + 15) & ~15;
-        const int t_begin = k0 + wave * per, t_end = min(k1, t_begin + per);
+        // The waves of a head take its keys in equal, consecutive shares.
+        const int heads = task[T_HEADS], shares = 4 / heads;
+        const int x = wave / shares;  // this wave's KV head, of the task's
+        const char* const kbase = static_cast<const char*>(a.k) + int64_t(kvh + x) * a.chs * EB;
+        const char* const vbase = static_cast<const char*>(a.v) + int64_t(kvh + x) * a.chs * EB;
+        const int per = ((k1 - k0 + shares - 1) / shares + 15) & ~15;
+        const int t_begin = k0 + (wave - x * shares) * per, t_end = min(k1, t_begin + per);
         if (t_begin < t_end) {
             // This lane's dims: E * col .. (DP 256: 8 * col .. and 128 + 8 * col ..);
             // lanes past the head's dims read dim 0 and write nothing.
@@ -701,7 +710,7 @@ shared_prefix_tasks(Args<T> a) {
             U16x8 qb[KS];  // B operand: query col, dims 32c + 8*quad ..
             {
                 int row, head;
-                query(q0 + min(col, qn - 1), row, head);
+                query(q0 + min(col, qn - 1), x, row, head);
                 const T* qrow = a.q + a.rows[row] * a.qts + head * a.qhs;
 #pragma unroll
                 for (int c = 0; c < KS; ++c) {
@@ -847,31 +856,27 @@ shared_prefix_tasks(Args<T> a) {
         }
         __syncthreads();
         constexpr int Q4 = DP / 4;
-        for (int x = tid; x < qn * Q4; x += kThreads) {
-            const int h = x / Q4, d = 4 * (x % Q4);
+        for (int i = tid; i < heads * qn * Q4; i += kThreads) {
+            const int y = i / (qn * Q4), h = i / Q4 - y * qn, d = 4 * (i % Q4);
             if (d >= D) continue;
-            float2 ml[4];
+            const int w0 = y * shares;  // the first of the head's waves
             float mx = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                ml[w] = sml[w * kNarrow + h];
-                mx = fmaxf(mx, ml[w].x);
-            }
+            for (int w = w0; w < w0 + shares; ++w) mx = fmaxf(mx, sml[w * kNarrow + h].x);
             const float m_use = mx == -INFINITY ? 0.f : mx;
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
             float l = 0.f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float f = __builtin_amdgcn_exp2f(ml[w].x - m_use);
+            for (int w = w0; w < w0 + shares; ++w) {
+                const float2 ml = sml[w * kNarrow + h];
+                const float f = __builtin_amdgcn_exp2f(ml.x - m_use);
                 const float4 p = *reinterpret_cast<const float4*>(so + (w * kNarrow + h) * DP + d);
-                l += f * ml[w].y;
+                l += f * ml.y;
                 sum.x += f * p.x;
                 sum.y += f * p.y;
                 sum.z += f * p.z;
                 sum.w += f * p.w;
             }
             int row, head;
-            query(q0 + h, row, head);
+            query(q0 + h, y, row, head);
             bool direct;
             const int64_t entry = entry_of(row, head, direct);
             if (direct) {
@@ -1065,6 +1070,14 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
             per = splits ? div_up(div_up(keys, splits), kKeyUnit) * kKeyUnit : 0;
             if (per) splits = div_up(keys, per);
         };
+        // KV heads of one task over a row's own keys: short ones share a task, a
+        // wave or two for each, so that its cost beside the keys is paid once.
+        auto heads_of = [&](int64_t keys, int64_t chunk) -> int64_t {
+            if (group > kNarrow) return 1;
+            for (int64_t h : {4, 2})
+                if (num_kv_heads % h == 0 && h * keys <= chunk) return h;
+            return 1;
+        };
         // The length of a task: the one that ends soonest by a simple estimate.
         // Tasks run on kSlots slots, longest first: all at once where they are
         // that few, otherwise the slots' mean share and half of a last, short
@@ -1089,7 +1102,10 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
                 if (g.prefix)
                     add(div_up(g.count * group, kWide) * num_kv_heads, g.count * num_heads, g.prefix);
             for (int64_t r = 0; r < num_rows; ++r)
-                if (own[r]) add(own_tiles * num_kv_heads, num_heads, own[r]);
+                if (own[r]) {
+                    const int64_t h = heads_of(own[r], c);
+                    add(own_tiles * num_kv_heads / h, num_heads, own[r] * h);
+                }
             const double time =
                 (count <= kSlots ? double(longest)
                                  : std::max(double(longest), double(sum) / kSlots +
@@ -1099,16 +1115,16 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
                 chunk = c;
                 best = time;
             }
-            if (c >= most) break;
+            if (c >= 4 * most) break;
         }
         int64_t n = 0;
-        auto emit = [&](int64_t member, int64_t q0, int64_t count, int64_t kvh, int64_t k0,
-                        int64_t k1, int64_t part) {
+        auto emit = [&](int64_t member, int64_t q0, int64_t count, int64_t kvh, int64_t heads,
+                        int64_t k0, int64_t k1, int64_t part) {
             int32_t* t = tasks + n++ * kTaskWords;
             t[T_MEMBER] = int32_t(member);
-            t[T_QBEGIN] = int32_t(q0);
-            t[T_QCOUNT] = int32_t(count);
+            t[T_QUERIES] = int32_t(q0 / kNarrow << 8 | count);
             t[T_KVH] = int32_t(kvh);
+            t[T_HEADS] = int32_t(heads);
             t[T_K0] = int32_t(k0);
             t[T_K1] = int32_t(k1);
             t[T_PART] = int32_t(part);
@@ -1141,7 +1157,7 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
                         const int64_t k0 = columns[c].split * gs[g].per;
                         const int64_t q0 = t * tile;
                         if (q0 < queries)
-                            emit(gs[g].first, q0, std::min(tile, queries - q0), columns[c].kvh, k0,
+                            emit(gs[g].first, q0, std::min(tile, queries - q0), columns[c].kvh, 1, k0,
                                  std::min(gs[g].prefix, k0 + gs[g].per), columns[c].split);
                     }
         }
@@ -1155,14 +1171,15 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
             const int64_t g = groups[r], shared = g >= 0 ? gs[g].splits : 0;
             const int64_t begin = g >= 0 ? gs[g].prefix : 0;
             int64_t splits, per;
+            const int64_t heads = heads_of(own[r], chunk);
             cut(own[r], chunk, splits, per);
             parts[r] = shared + splits;
             for (int64_t s = 0; s < splits; ++s)
                 for (int64_t t = 0; t < own_tiles; ++t)
-                    for (int64_t h = 0; h < num_kv_heads; ++h) {
+                    for (int64_t h = 0; h < num_kv_heads; h += heads) {
                         const int64_t k0 = begin + s * per;
                         emit(place[r], t * kWide, std::min<int64_t>(kWide, group - t * kWide), h,
-                             k0, std::min(lengths[r], k0 + per), shared + s);
+                             heads, k0, std::min(lengths[r], k0 + per), shared + s);
                     }
         }
         int64_t entries = 0;

@@ -25,8 +25,8 @@
 namespace tvllm {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kPer = 8;                  // tokens per thread
+constexpr int kThreads = 512;
+constexpr int kPer = 16;                 // tokens per thread
 constexpr int kSpan = kThreads * kPer;   // tokens per workgroup
 constexpr uint32_t kPrompt = 0x80000000u;  // the token stands in the prompt part
 
@@ -35,7 +35,7 @@ struct Args {
     void* out;
     int64_t stride, out_stride;  // elements
     int64_t vocab, spans, grid;
-    bool in_place;
+    bool in_place, list4;  // list4: the history's rows are 16-byte aligned
     const float* repetition;
     const float* presence;
     const float* frequency;
@@ -54,65 +54,56 @@ struct Args {
     const int64_t* mask_rows;
 };
 
-// VEC: rows of both tensors are 16-byte aligned, a thread's tokens are 8
+// VEC: rows of both tensors are 16-byte aligned, a thread's tokens are runs of 8
 // neighbours; otherwise neighbouring threads hold neighbouring tokens.
 template <typename TI, typename TO, bool VEC>
 __global__ void __launch_bounds__(kThreads)
 logit_controls(Args a) {
-    __shared__ uint32_t count[kSpan];
+    __shared__ __align__(16) uint32_t count[kSpan];
     const int tid = threadIdx.x;
     int64_t bid = blockIdx.x;
     // Block ids are dealt to 8 XCDs in turn: give each a contiguous range.
-    const int64_t per = a.grid / 8, rest = a.grid % 8, xcd = bid % 8;
-    bid = xcd * per + min(xcd, rest) + bid / 8;
+    const int64_t share = a.grid / 8, rest = a.grid % 8, xcd = bid % 8;
+    bid = xcd * share + min(xcd, rest) + bid / 8;
     const int64_t r = bid / a.spans;
     const int64_t base = (bid - r * a.spans) * kSpan;
     const int64_t left = a.vocab - base;  // tokens of the span
-    auto at = [&](int e) { return VEC ? tid * kPer + e : e * kThreads + tid; };
+    auto at = [&](int e) {
+        return VEC ? (e / 8 * kThreads + tid) * 8 + e % 8 : e * kThreads + tid;
+    };
 
-    // What the row asks for (all uniform).
-    int64_t slot = a.history ? a.slots[r] : -1, n = 0, prompt = 0;
-    float rho = 1.f, pres = 0.f, freq = 0.f;
-    if (slot >= 0 && slot < a.num_slots) {
-        n = a.lengths[r];
-        prompt = a.prompts[r];
-        if (a.repetition) rho = a.repetition[r];
-        if (a.presence) pres = a.presence[r];
-        if (a.frequency) freq = a.frequency[r];
-    }
-    int32_t* const list = a.history + (n > 0 ? slot * a.capacity : 0);
-    // The newest token: it takes the last position, which nobody reads here.
-    int64_t last = -1;
-    if (n > 0 && a.newest) {
-        last = a.newest[r];
-        if (last < 0 || last >= a.vocab) last = -1;
-        --n;
-        if (base == 0 && tid == 0 && n < a.capacity) list[n] = int32_t(last);
-    }
-    const int64_t stored = min(n, a.capacity);
-    const bool penal = (stored > 0 || last >= 0) && (rho != 1.f || pres != 0.f || freq != 0.f);
-    int64_t b0 = 0, b1 = 0;
-    if (a.bias_offsets) {
-        b0 = max(int64_t(0), a.bias_offsets[r]);
-        b1 = min(a.num_bias, a.bias_offsets[r + 1]);
-    }
-    const bool biased = b0 < b1;
+    // What the row asks for: all uniform, and all loaded at once.
+    int64_t slot = a.history ? a.slots[r] : -1;
+    int64_t n = a.history ? a.lengths[r] : 0, prompt = a.history ? a.prompts[r] : 0;
+    const float rho = a.repetition ? a.repetition[r] : 1.f;
+    const float pres = a.presence ? a.presence[r] : 0.f;
+    const float freq = a.frequency ? a.frequency[r] : 0.f;
+    int64_t last = a.newest ? a.newest[r] : -1;
+    int64_t b0 = a.bias_offsets ? a.bias_offsets[r] : 0;
+    int64_t b1 = a.bias_offsets ? a.bias_offsets[r + 1] : 0;
     const int64_t mrow = a.mask_rows ? a.mask_rows[r] : -1;
-    const bool masked = mrow >= 0 && mrow < a.mask_count;
-    if (a.in_place && !penal && !biased && !masked) return;
-
     const TI* const src = static_cast<const TI*>(a.logits) + r * a.stride + base;
     TO* const dst = static_cast<TO*>(a.out) + r * a.out_stride + base;
     float x[kPer];
     auto load = [&]() {
-        if (VEC && at(0) + kPer <= left) {
-            if constexpr (sizeof(TI) == 2) {
-                unpack8<TI>(*reinterpret_cast<const U16x8*>(src + at(0)), x);
-            } else {
-                const float4 lo = *reinterpret_cast<const float4*>(src + at(0));
-                const float4 hi = *reinterpret_cast<const float4*>(src + at(0) + 4);
-                x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w;
-                x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int g = 0; g < kPer / 8; ++g) {
+                float (&y)[8] = reinterpret_cast<float (&)[8]>(x[8 * g]);
+                if (at(8 * g) + 8 <= left) {
+                    if constexpr (sizeof(TI) == 2) {
+                        unpack8<TI>(*reinterpret_cast<const U16x8*>(src + at(8 * g)), y);
+                    } else {
+                        const float4 lo = *reinterpret_cast<const float4*>(src + at(8 * g));
+                        const float4 hi = *reinterpret_cast<const float4*>(src + at(8 * g) + 4);
+                        y[0] = lo.x; y[1] = lo.y; y[2] = lo.z; y[3] = lo.w;
+                        y[4] = hi.x; y[5] = hi.y; y[6] = hi.z; y[7] = hi.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        y[e] = at(8 * g + e) < left ? to_f<TI>(src[at(8 * g + e)]) : 0.f;
+                }
             }
         } else {
 #pragma unroll
@@ -122,28 +113,88 @@ logit_controls(Args a) {
     // Out of place every token is copied: the loads go out ahead of the counting.
     if (!a.in_place) load();
 
+    if (slot < 0 || slot >= a.num_slots || n <= 0) {
+        n = 0;
+        last = -1;
+        slot = 0;
+    }
+    int32_t* const list = a.history + slot * a.capacity;
+    // The newest token: it takes the last position, which nobody reads here.
+    if (n > 0 && a.newest) {
+        if (last < 0 || last >= a.vocab) last = -1;
+        --n;
+        if (base == 0 && tid == 0 && n < a.capacity) list[n] = int32_t(last);
+    }
+    const int stored = int(min(n, a.capacity));
+    const bool penal = (stored > 0 || last >= 0) && (rho != 1.f || pres != 0.f || freq != 0.f);
+    b0 = max(int64_t(0), b0);
+    b1 = min(a.num_bias, b1);
+    const bool biased = b0 < b1;
+    const bool masked = mrow >= 0 && mrow < a.mask_count;
+    if (a.in_place && !penal && !biased && !masked) return;
+
+    // A thread reads its tokens' counts where it keeps the tokens themselves.
     uint32_t c[kPer] = {};
     uint32_t which[kPer] = {};  // 1 + the token's last entry in the row's biases
     auto clear = [&]() {
-        for (int i = tid; i < kSpan; i += kThreads) count[i] = 0u;
+#pragma unroll
+        for (int i = 0; i < kPer / 4; ++i)
+            reinterpret_cast<uint4*>(count)[i * kThreads + tid] = make_uint4(0, 0, 0, 0);
         __syncthreads();
     };
     auto read = [&](uint32_t (&to)[kPer]) {
         __syncthreads();
+        if constexpr (VEC) {
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) to[e] = count[at(e)];
+            for (int i = 0; i < kPer / 4; ++i) {
+                const uint4 w = *reinterpret_cast<const uint4*>(&count[at(4 * i)]);
+                to[4 * i] = w.x;
+                to[4 * i + 1] = w.y;
+                to[4 * i + 2] = w.z;
+                to[4 * i + 3] = w.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) to[e] = count[at(e)];
+        }
     };
     if (penal) {
         clear();
-        auto add = [&](int64_t token, int64_t position) {
-            const int64_t i = token - base;
-            if (i >= 0 && i < kSpan) {
-                if (position < prompt) atomicOr(&count[i], kPrompt);
+        const uint32_t low = uint32_t(base);
+        const int64_t split = prompt;
+        auto add = [&](int32_t token, int position) {
+            const uint32_t i = uint32_t(token) - low;  // (ids below the span wrap past it)
+            if (i < uint32_t(kSpan)) {
+                if (position < split) atomicOr(&count[i], kPrompt);
                 else atomicAdd(&count[i], 1u);
             }
         };
-        for (int64_t p = tid; p < stored; p += kThreads) add(list[p], p);
-        if (tid == 0 && last >= 0) add(last, n);
+        // Several loads of a thread at once, of four ids each where the list's
+        // rows are aligned.
+        constexpr int kAhead = 4;
+        int p = 0;
+        if (a.list4) {
+            const int4* const list4 = reinterpret_cast<const int4*>(list);
+            for (; p + 4 <= stored; p += 4 * kAhead * kThreads) {
+                int4 t[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const int q = p / 4 + k * kThreads + tid;
+                    t[k] = 4 * q + 4 <= stored ? list4[q] : make_int4(-1, -1, -1, -1);
+                }
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const int q = p + 4 * (k * kThreads + tid);
+                    add(t[k].x, q);
+                    add(t[k].y, q + 1);
+                    add(t[k].z, q + 2);
+                    add(t[k].w, q + 3);
+                }
+            }
+            p = stored & ~3;
+        }
+        for (p += tid; p < stored; p += kThreads) add(list[p], p);
+        if (tid == 0 && last >= 0) add(int32_t(last), int(min(n, int64_t(INT32_MAX))));
         read(c);
     }
     if (biased) {
@@ -158,40 +209,68 @@ logit_controls(Args a) {
 
     bool touched = masked;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) touched |= c[e] != 0u || which[e] != 0u;
+    for (int e = 0; e < kPer; ++e) touched |= (c[e] | which[e]) != 0u;
     if (a.in_place) {
         if (!touched) return;
         load();
     }
     if (touched) {
+        if (penal) {
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            if (c[e]) {
-                x[e] = x[e] > 0.f ? x[e] / rho : x[e] * rho;
-                const uint32_t times = c[e] & ~kPrompt;
-                x[e] -= freq * float(times);
-                if (times) x[e] -= pres;
-            }
-            if (which[e]) x[e] += a.bias_values[b0 + which[e] - 1];
+            for (int e = 0; e < kPer; ++e)
+                if (c[e]) {
+                    x[e] = x[e] > 0.f ? x[e] / rho : x[e] * rho;
+                    const uint32_t times = c[e] & ~kPrompt;
+                    x[e] -= freq * float(times);
+                    if (times) x[e] -= pres;
+                }
+        }
+        if (biased) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+                if (which[e]) x[e] += a.bias_values[b0 + which[e] - 1];
         }
         if (masked) {
             const uint32_t* const words = a.mask + mrow * a.mask_stride;
+            if constexpr (VEC) {
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                const int64_t i = base + at(e);
-                if (at(e) < left && !((words[i >> 5] >> (i & 31)) & 1u)) x[e] = -INFINITY;
+                for (int g = 0; g < kPer / 8; ++g)
+                    if (at(8 * g) < left) {
+                        const int64_t i = base + at(8 * g);
+                        const uint32_t bits = words[i >> 5] >> (i & 31);  // 8 of one word
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (!((bits >> e) & 1u)) x[8 * g + e] = -INFINITY;
+                    }
+            } else {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) {
+                    const int64_t i = base + at(e);
+                    if (at(e) < left && !((words[i >> 5] >> (i & 31)) & 1u)) x[e] = -INFINITY;
+                }
             }
         }
     }
-    if (VEC && at(0) + kPer <= left) {
-        if constexpr (sizeof(TO) == 2) {
-            U16x8 w;
+    if constexpr (VEC) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w.w[e] = pack2<TO>(x[2 * e], x[2 * e + 1]);
-            *reinterpret_cast<U16x8*>(dst + at(0)) = w;
-        } else {
-            *reinterpret_cast<float4*>(dst + at(0)) = make_float4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<float4*>(dst + at(0) + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        for (int g = 0; g < kPer / 8; ++g) {
+            const float (&y)[8] = reinterpret_cast<const float (&)[8]>(x[8 * g]);
+            TO* const to = dst + at(8 * g);
+            if (at(8 * g) + 8 <= left) {
+                if constexpr (sizeof(TO) == 2) {
+                    U16x8 w;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w.w[e] = pack2<TO>(y[2 * e], y[2 * e + 1]);
+                    *reinterpret_cast<U16x8*>(to) = w;
+                } else {
+                    *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<float4*>(to + 4) = make_float4(y[4], y[5], y[6], y[7]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (at(8 * g + e) < left) to[e] = static_cast<TO>(y[e]);
+            }
         }
     } else {
 #pragma unroll
@@ -246,6 +325,7 @@ extern "C" int tvllm_logit_controls(
     a.spans = (vocab + kSpan - 1) / kSpan;
     a.grid = rows * a.spans;
     a.in_place = logits == out;
+    a.list4 = aligned16(history) && capacity % 4 == 0;
     a.repetition = repetition;
     a.presence = presence;
     a.frequency = frequency;

@@ -12,7 +12,7 @@ from tinyvllm.kernels.sampling import _check_logits
 
 
 def _ptr(tensor: torch.Tensor | None) -> int | None:
-    return None if tensor is None or tensor.numel() == 0 else tensor.data_ptr()
+    return None if tensor is None else tensor.data_ptr() or None  # (0: empty)
 
 
 def apply_logit_controls(
@@ -59,37 +59,22 @@ def apply_logit_controls(
     _check_logits(logits)
     rows, vocab = logits.shape
     device = require_gpu(logits)
+    index = device.index
     if out is None:
         out = torch.empty((rows, vocab), dtype=logits.dtype, device=device)
     elif (out.shape != logits.shape or out.stride(1) != 1
           or out.dtype not in (logits.dtype, torch.float32)):
         raise RuntimeError("out must be float32 or of the logits' type, of their shape, with "
                            "unit last stride")
-    for name, tensor, dtype, size in (
-            ("repetition", repetition, torch.float32, rows),
-            ("presence", presence, torch.float32, rows),
-            ("frequency", frequency, torch.float32, rows),
-            ("slots", slots, torch.long, rows), ("lengths", lengths, torch.long, rows),
-            ("prompt_lens", prompt_lens, torch.long, rows),
-            ("newest", newest, torch.long, rows), ("mask_rows", mask_rows, torch.long, rows),
-            ("bias_offsets", bias_offsets, torch.long, rows + 1),
-            ("bias_tokens", bias_tokens, torch.int32, None),
-            ("bias_values", bias_values, torch.float32, None)):
-        if tensor is None:
-            continue
-        if tensor.dtype != dtype or tensor.dim() != 1 or not tensor.is_contiguous() or (
-                size is not None and tensor.numel() != size):
-            raise RuntimeError(f"{name} must be a contiguous {dtype} vector"
-                               + ("" if size is None else f" of {size}"))
-        require_gpu(logits, tensor)
-    if history is not None:
-        if slots is None or lengths is None or prompt_lens is None:
-            raise RuntimeError("a history needs slots, lengths and prompt_lens")
-        if history.dtype != torch.int32 or history.dim() != 2 or not history.is_contiguous():
-            raise RuntimeError("history must be contiguous int32 [slots, capacity]")
-        require_gpu(logits, history)
-    elif any(t is not None for t in (repetition, presence, frequency, newest)):
-        raise RuntimeError("penalties need a history")
+    elif out.get_device() != index:
+        raise RuntimeError("tensors must share one GPU device")
+    if history is None:
+        if not (repetition is presence is frequency is newest is None):
+            raise RuntimeError("penalties need a history")
+    elif slots is None or lengths is None or prompt_lens is None:
+        raise RuntimeError("a history needs slots, lengths and prompt_lens")
+    elif history.dtype != torch.int32 or history.dim() != 2 or not history.is_contiguous():
+        raise RuntimeError("history must be contiguous int32 [slots, capacity]")
     if (bias_offsets is None) != (bias_tokens is None) or (bias_tokens is None) != (
             bias_values is None):
         raise RuntimeError("biases need tokens, values and offsets")
@@ -97,13 +82,31 @@ def apply_logit_controls(
         raise RuntimeError("bias_tokens and bias_values must align")
     if (mask is None) != (mask_rows is None):
         raise RuntimeError("masks need mask_rows")
-    if mask is not None:
-        if mask.dtype != torch.int32 or mask.dim() != 2 or mask.stride(1) != 1 or (
-                mask.shape[0] and mask.shape[1] < -(-vocab // 32)):
-            raise RuntimeError("mask must be int32 [masks, words] with unit last stride and a "
-                               "bit for every token")
-        require_gpu(logits, mask)
-    require_gpu(logits, out)
+    if mask is not None and (mask.dtype != torch.int32 or mask.dim() != 2 or mask.stride(1) != 1
+                             or (mask.shape[0] and mask.shape[1] < -(-vocab // 32))):
+        raise RuntimeError("mask must be int32 [masks, words] with unit last stride and a bit "
+                           "for every token")
+    for tensor in (history, mask):
+        if tensor is not None and tensor.get_device() != index:
+            raise RuntimeError("tensors must share one GPU device")
+    for names, dtype, size, tensors in (
+            (("repetition", "presence", "frequency"), torch.float32, rows,
+             (repetition, presence, frequency)),
+            (("slots", "lengths", "prompt_lens", "newest", "mask_rows"), torch.long, rows,
+             (slots, lengths, prompt_lens, newest, mask_rows)),
+            (("bias_offsets",), torch.long, rows + 1, (bias_offsets,)),
+            (("bias_tokens",), torch.int32, None, (bias_tokens,)),
+            (("bias_values",), torch.float32, None, (bias_values,))):
+        for name, tensor in zip(names, tensors):
+            if tensor is None:
+                continue
+            shape = tensor.shape
+            if tensor.dtype != dtype or len(shape) != 1 or not tensor.is_contiguous() or (
+                    size is not None and shape[0] != size):
+                raise RuntimeError(f"{name} must be a contiguous {dtype} vector"
+                                   + ("" if size is None else f" of {size}"))
+            if tensor.get_device() != index:
+                raise RuntimeError("tensors must share one GPU device")
     if rows == 0:
         return out
     check(load_kernels().tvllm_logit_controls(

@@ -211,7 +211,8 @@ int tvllm_paged_decode_noalloc(const void* q, int64_t q_token_stride,
  * host (no GPU call) and fills `plan`, a host buffer of at least
  * tvllm_shared_prefix_plan_words int32 words, which the caller copies to the
  * device; one plan serves every layer of a step.
- *   lengths[r] is row r's context (0: padding, its output is zeros);
+ *   lengths[r] is row r's context (0: padding, its output is zeros; at most
+ *     2^31 - 4097 tokens);
  *   groups[r] its group, or -1; the first prefix_lens[g] tokens (whole blocks)
  *   of every row of group g lie in the same blocks, the rows' tables naming
  *   them alike. lengths[r] >= prefix_lens[groups[r]]. A group of one row

@@ -68,6 +68,7 @@ enum Task { T_MEMBER, T_QUERIES, T_KVH, T_HEADS, T_K0, T_K1, T_PART, T_ROW };
 constexpr int64_t kSlots = 512;     // workgroups at once: two on each of 256 CUs
 constexpr int64_t kKeyUnit = 64;    // tasks' key ranges are multiples of this
 constexpr int64_t kMaxParts = 64;   // splits of one unit
+constexpr int64_t kMaxContext = INT32_MAX - 4096;  // token numbers past a tile's end fit in 32 bits
 constexpr int64_t kMaxSplits = 1024;  // tasks that splitting adds, all units together
 // What a task costs beside its keys (its chain of first loads, the merge in LDS
 // and the write of its part), in keys.
@@ -1022,7 +1023,7 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
     TVLLM_CHECK(num_rows == 0 || (lengths && groups), "shared_prefix_plan: null pointer");
     TVLLM_CHECK(num_groups == 0 || prefix_lens, "shared_prefix_plan: null pointer");
     for (int64_t g = 0; g < num_groups; ++g)
-        TVLLM_CHECK(prefix_lens[g] >= 0 && prefix_lens[g] <= INT32_MAX &&
+        TVLLM_CHECK(prefix_lens[g] >= 0 && prefix_lens[g] <= kMaxContext &&
                         prefix_lens[g] % block_size == 0,
                     "shared_prefix_plan: prefix lengths must be whole blocks");
     const int64_t group = num_heads / num_kv_heads;
@@ -1032,7 +1033,7 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
     try {
         std::vector<Group> gs(static_cast<size_t>(num_groups));
         for (int64_t r = 0; r < num_rows; ++r) {
-            TVLLM_CHECK(lengths[r] >= 0 && lengths[r] <= INT32_MAX,
+            TVLLM_CHECK(lengths[r] >= 0 && lengths[r] <= kMaxContext,
                         "shared_prefix_plan: invalid context length");
             TVLLM_CHECK(groups[r] >= -1 && groups[r] < num_groups,
                         "shared_prefix_plan: group index out of range");

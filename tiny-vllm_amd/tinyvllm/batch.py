@@ -111,6 +111,10 @@ class PreparedBatch:
     # (equal epochs: the table only grew since). None: upload whole tables.
     request_slots: tuple[int, ...] | None = None
     kv_table_epochs: tuple[int, ...] | None = None
+    # Logit controls (beyond the reference): per sampled row, None or the
+    # request's (prompt ids, answer ids), its own live lists; the newest answer
+    # id may be a negative placeholder. None: no sampled request has controls.
+    sample_histories: tuple | None = None
 
     @property
     def num_items(self) -> int:
@@ -184,6 +188,7 @@ class BatchBuilder:
         sample_idx: list[int] = []
         sample_rid: list[int] = []
         params: list[SamplingParams] = []
+        histories: list = []
         tables: list[np.ndarray] = []
         table_off = [0]
         epoch_of = getattr(kv, "table_epoch", None)
@@ -227,6 +232,8 @@ class BatchBuilder:
                 sample_idx.append(q_offsets[-1] - 1)
                 sample_rid.append(item.request_id)
                 params.append(request.sampling)
+                histories.append((request.prompt_token_ids, request.output_token_ids)
+                                 if request.sampling.controlled else None)
         return PreparedBatch(
             plan_id=plan.plan_id, mode=plan.mode,
             input_ids=tuple(input_ids), positions=tuple(positions),
@@ -243,4 +250,6 @@ class BatchBuilder:
             request_slots=tuple(i.request_slot for i in plan.items),
             kv_table_epochs=None if epoch_of is None else tuple(
                 epoch_of(i.request_id) for i in plan.items),
+            sample_histories=tuple(histories) if any(
+                h is not None for h in histories) else None,
         )

@@ -26,7 +26,9 @@ class EngineConfig:
     heads, dim] cache view ("auto": head-major for fewer than 256 (request,
     KV head) pairs, token-major otherwise); ``prefill_graph_tokens`` the
     largest prefill/mixed step replayed from a captured graph (None: sized
-    from the model, 0: prefill always eager)."""
+    from the model, 0: prefill always eager); ``shared_prefix_attention`` has
+    decode steps take cached pages that many requests share once for all of
+    them (hip backend)."""
 
     model: Path
     dtype: DType = "bfloat16"
@@ -47,6 +49,7 @@ class EngineConfig:
     kv_v_scale: float = 1.0
     kv_cache_layout: str = "auto"
     prefill_graph_tokens: int | None = None
+    shared_prefix_attention: bool = False
 
     def __post_init__(self) -> None:
         model = Path(self.model).expanduser().resolve()
@@ -71,7 +74,7 @@ class EngineConfig:
         graph_tokens = self.prefill_graph_tokens
         if graph_tokens is not None and (type(graph_tokens) is not int or graph_tokens < 0):
             raise ValueError("prefill_graph_tokens must be None or a non-negative int")
-        for name in ("enforce_eager", "enable_prefix_caching"):
+        for name in ("enforce_eager", "enable_prefix_caching", "shared_prefix_attention"):
             if type(getattr(self, name)) is not bool:
                 raise TypeError(f"{name} must be bool")
         for name in ("max_model_len", "max_num_seqs", "max_num_batched_tokens",

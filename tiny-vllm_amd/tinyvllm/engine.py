@@ -149,6 +149,7 @@ class Engine:
                 raise TypeError("requests must contain GenerateRequest values")
             self.scheduler.validate_request(spec.prompt_token_ids, spec.sampling)
             self.executor.capabilities.validate_token_ids(spec.prompt_token_ids)
+            self.executor.capabilities.validate_token_ids(spec.sampling.control_token_ids)
             arrival = self._clock() if spec.arrival_ns is None else spec.arrival_ns
             _check_non_negative_int("arrival_ns", arrival)
             rid = next_id if spec.request_id is None else spec.request_id

@@ -84,14 +84,16 @@ class Executor:
                  kv_cache_dtype: torch.dtype | None = None,
                  kv_scales: tuple[float, float] = (1.0, 1.0),
                  kv_cache_layout: str = "auto",
-                 prefill_graph_tokens: int | None = None) -> None:
+                 prefill_graph_tokens: int | None = None,
+                 shared_prefix_attention: bool = False) -> None:
         self.runner = ModelRunner(model, block_size=block_size, num_blocks=num_blocks,
                                   max_model_len=max_model_len, max_num_seqs=max_num_seqs,
                                   attention_backend=attention_backend,
                                   enforce_eager=enforce_eager, graph_sizes=graph_sizes,
                                   kv_cache_dtype=kv_cache_dtype, kv_scales=kv_scales,
                                   kv_cache_layout=kv_cache_layout,
-                                  prefill_graph_tokens=prefill_graph_tokens)
+                                  prefill_graph_tokens=prefill_graph_tokens,
+                                  shared_prefix_attention=shared_prefix_attention)
         self.capabilities = ExecutorCapabilities(
             vocab_size=model.config.vocab_size,
             max_model_len=self.runner.max_model_len,
@@ -141,6 +143,7 @@ class Executor:
 
     def release(self, request_id: int) -> None:
         self.sampler.release(request_id)
+        self.runner.release(request_id)
 
     def clear(self) -> None:
         try:

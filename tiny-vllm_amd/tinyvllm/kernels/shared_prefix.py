@@ -99,6 +99,33 @@ class SharedPrefixPlan:
         self.workspace_bytes = need.value
 
 
+def find_shared_prefixes(table_ids, table_offsets, context_lens, block_size: int
+                         ) -> tuple[np.ndarray, np.ndarray]:
+    """(group of each row or -1, prefix tokens of each group) of a batch whose
+    row r's block ids are ``table_ids[table_offsets[r]:table_offsets[r + 1]]``:
+    rows with the same first block form a group, whose prefix is the longest
+    run of leading blocks that they all have, the block of a row's newest token
+    (which the step writes) left out."""
+    ids = np.asarray(table_ids, dtype=np.int64)
+    offsets = np.asarray(table_offsets, dtype=np.int64)
+    lengths = np.asarray(context_lens, dtype=np.int64)
+    groups = np.full(len(lengths), -1, dtype=np.int64)
+    usable = np.maximum(lengths - 1, 0) // block_size
+    rows = np.flatnonzero(usable)
+    prefixes = []
+    if len(rows) > 1:
+        _, inverse, counts = np.unique(ids[offsets[rows]], return_inverse=True,
+                                       return_counts=True)
+        for g in np.flatnonzero(counts > 1):
+            members = rows[inverse == g]
+            common = int(usable[members].min())
+            tables = ids[offsets[members][:, None] + np.arange(common)]
+            differ = np.flatnonzero((tables != tables[0]).any(axis=0))
+            groups[members] = len(prefixes)
+            prefixes.append((int(differ[0]) if len(differ) else common) * block_size)
+    return groups, np.asarray(prefixes, dtype=np.int64)
+
+
 def paged_decode_shared_prefix(
     q: torch.Tensor,
     cache: PagedKVCache,

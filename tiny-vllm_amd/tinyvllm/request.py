@@ -6,10 +6,13 @@ user code written against it keep working.
 from __future__ import annotations
 
 import math
+from collections.abc import Iterable, Mapping
 from dataclasses import dataclass, field
 from enum import Enum, auto
 
-from tinyvllm._validation import _check_non_negative_int, _check_token_id
+from tinyvllm._validation import (
+    _check_non_negative_int, _check_token_id, _normalize_token_ids,
+)
 
 _MAX_SEED = (1 << 64) - 1
 
@@ -33,7 +36,14 @@ class WorkClass(Enum):
 
 @dataclass(frozen=True, slots=True)
 class SamplingParams:
-    """Per-request decoding policy. temperature 0 means greedy."""
+    """Per-request decoding policy. temperature 0 means greedy.
+
+    Beyond the reference, controls applied to the logits before sampling, in
+    this order: tokens of the prompt or the answer so far have positive logits
+    divided by ``repetition_penalty`` and others multiplied by it; tokens of the
+    answer lose ``frequency_penalty`` for each time they stand in it and
+    ``presence_penalty`` once; ``logit_bias`` (a mapping, kept as sorted pairs)
+    is added; only ``allowed_token_ids`` (None: all) can be drawn."""
 
     max_new_tokens: int = 64
     temperature: float = 0.0
@@ -41,6 +51,11 @@ class SamplingParams:
     seed: int = 0
     top_k: int = 0
     top_p: float = 1.0
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: Mapping[int, float] | tuple[tuple[int, float], ...] = ()
+    allowed_token_ids: Iterable[int] | frozenset[int] | None = None
 
     def __post_init__(self) -> None:
         _check_non_negative_int("max_new_tokens", self.max_new_tokens)
@@ -64,10 +79,50 @@ class SamplingParams:
         object.__setattr__(self, "top_p", top_p)
         if type(self.ignore_eos) is not bool:
             raise TypeError("ignore_eos must be bool")
+        for name in ("repetition_penalty", "presence_penalty", "frequency_penalty"):
+            object.__setattr__(self, name, _float32(name, getattr(self, name)))
+        if self.repetition_penalty <= 0.0:
+            raise ValueError("repetition_penalty must be positive")
+        bias = self.logit_bias
+        pairs = dict(bias.items() if isinstance(bias, Mapping) else bias)
+        for token_id in pairs:
+            _check_token_id(token_id)
+        object.__setattr__(self, "logit_bias", tuple(
+            (token_id, _float32("logit_bias", pairs[token_id])) for token_id in sorted(pairs)))
+        if self.allowed_token_ids is not None:
+            allowed = _normalize_token_ids("allowed_token_ids", self.allowed_token_ids)
+            if not allowed:
+                raise ValueError("allowed_token_ids must name a token")
+            object.__setattr__(self, "allowed_token_ids", allowed)
 
     @property
     def greedy(self) -> bool:
         return self.temperature == 0.0
+
+    @property
+    def penalised(self) -> bool:
+        """Whether the logits depend on the request's tokens so far."""
+        return (self.repetition_penalty != 1.0 or self.presence_penalty != 0.0
+                or self.frequency_penalty != 0.0)
+
+    @property
+    def controlled(self) -> bool:
+        """Whether the logits are changed before sampling."""
+        return bool(self.logit_bias) or self.allowed_token_ids is not None or self.penalised
+
+    @property
+    def control_token_ids(self) -> tuple[int, ...]:
+        """Tokens that the controls name (they must lie in the vocabulary)."""
+        return tuple(t for t, _ in self.logit_bias) + tuple(self.allowed_token_ids or ())
+
+
+def _float32(name: str, value: float) -> float:
+    """A number that is finite in float32, which the controls compute in."""
+    if type(value) not in (int, float):
+        raise TypeError(f"{name} must be a number")
+    if not abs(value) <= 3.4028234663852886e38:  # (also: not NaN)
+        raise ValueError(f"{name} must be finite")
+    return float(value)
 
 
 @dataclass(slots=True)

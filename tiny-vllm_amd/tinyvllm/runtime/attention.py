@@ -9,6 +9,8 @@
   * decode rows (query length 1): split-K paged decode attention;
   * multi-query rows (fresh prompts and chunks with history): MFMA paged
     prefill attention, reading the just-written chunk from the cache too;
+  * decode-only steps by a ``SharedPrefixPlan``: QK-norm + RoPE with the KV
+    write, then decode attention that takes the keys which rows share once;
   * other head dims (up to 256; the reference dispatches 32, 64, 128, 256)
     and GQA groups above 16 take the same calls, served by the library's
     general_attention.hip (MFMA kernels for those four head dims).
@@ -29,6 +31,7 @@ from tinyvllm.kernels.paged_decode import (
 )
 from tinyvllm.kernels.paged_prefill import paged_prefill_attention
 from tinyvllm.kernels.pointwise import qk_norm_rope, qk_norm_rope_store
+from tinyvllm.kernels.shared_prefix import SharedPrefixPlan, paged_decode_shared_prefix
 from tinyvllm.paged_kv import PagedKVCache
 from tinyvllm.runtime.contracts import ModelInput
 
@@ -39,10 +42,16 @@ class HipAttention:
     """Fused KV write, paged decode and paged chunked prefill on HIP kernels."""
 
     def __init__(self, model_input: ModelInput, cache: PagedKVCache, *,
-                 decode_workspace: torch.Tensor | None = None) -> None:
+                 decode_workspace: torch.Tensor | None = None,
+                 shared_prefix: SharedPrefixPlan | None = None,
+                 shared_workspace: torch.Tensor | None = None) -> None:
+        """``shared_prefix``: the plan that decode rows follow (its context
+        lengths are theirs), with its workspace."""
         self.kv = model_input.kv
         self.cache = cache
         self.decode_workspace = decode_workspace
+        self.shared_prefix = shared_prefix
+        self.shared_workspace = shared_workspace
         self._written_layer = -1
         self._fused = None
 
@@ -50,7 +59,10 @@ class HipAttention:
         """Decode-only steps whose shape the fused decode kernel takes (head
         dim 128, GQA group <= 16): QK-norm + RoPE + KV write + attention in
         one launch. Other head dims run the unfused kernels (QK-norm + RoPE
-        with the KV write, then the general paged-attention kernel)."""
+        with the KV write, then the general paged-attention kernel), and so do
+        steps by a shared-prefix plan."""
+        if self.shared_prefix is not None:
+            return False
         group = num_heads // self.cache.num_kv_heads
         return (self.kv.prefill is None and self.kv.decode is not None
                 and self.cache.head_dim == 128 and 1 <= group <= 16)
@@ -101,7 +113,11 @@ class HipAttention:
             return output
         if self._written_layer != layer_idx:
             store_kv(self.cache, layer_idx, self.kv.slot_mapping, k, v)
-        if self.kv.decode is not None:
+        if self.kv.decode is not None and self.shared_prefix is not None:
+            paged_decode_shared_prefix(q, self.cache, layer_idx, self.kv.decode,
+                                       self.shared_prefix, output, scale=scale,
+                                       workspace=self.shared_workspace)
+        elif self.kv.decode is not None:
             paged_decode_attention(q, self.cache, layer_idx, self.kv.decode, output,
                                    scale=scale, workspace=self.decode_workspace)
         if self.kv.prefill is not None:

@@ -18,6 +18,7 @@ import torch
 from tinyvllm.kernels.kv_store import begin_decode
 from tinyvllm.kernels.paged_decode import decode_split_plan
 from tinyvllm.kernels.sampling import sample
+from tinyvllm.kernels.shared_prefix import SharedPrefixPlan
 from tinyvllm.paged_kv import PagedKVCache
 from tinyvllm.runtime.attention import HipAttention
 from tinyvllm.runtime.inputs import DecodeInputs
@@ -50,6 +51,8 @@ class DecodeGraphs:
         # size -> [(context bound, graph, logits, tokens)] ascending by bound
         self.entries: dict[int, list[tuple[int, torch.cuda.CUDAGraph, torch.Tensor,
                                            torch.Tensor]]] = {}
+        # size -> (graph, logits, tokens) of steps by a shared-prefix plan
+        self.shared: dict[int, tuple[torch.cuda.CUDAGraph, torch.Tensor, torch.Tensor]] = {}
         self.tokens: torch.Tensor | None = None
         self.pool = None
 
@@ -57,12 +60,15 @@ class DecodeGraphs:
     def capture(self, model: torch.nn.Module, inputs: DecodeInputs, cache: PagedKVCache,
                 workspace: torch.Tensor | None, *,
                 sizes: tuple[int, ...] | None = None,
-                tokens: torch.Tensor | None = None) -> None:
+                tokens: torch.Tensor | None = None,
+                shared_prefix: SharedPrefixPlan | None = None,
+                shared_workspace: torch.Tensor | None = None) -> None:
         """Capture one graph per bucket size (default: ``bucket_sizes`` up to
         the input capacity). ``tokens`` (int64, >= capacity rows) receives
         every replay's sampled ids; a replay first takes its input ids from
         the previous step's rows there wherever the uploaded token sources
-        say so."""
+        say so. ``shared_prefix``: capture each size above 1 once more, by that
+        plan (a replay follows what the plan then holds)."""
         limit = min(inputs.capacity, cache.num_blocks)
         sizes = bucket_sizes(limit) if sizes is None else tuple(
             sorted({min(int(x), limit) for x in sizes}))
@@ -92,6 +98,10 @@ class DecodeGraphs:
                 for size in reversed(sizes):
                     for bound in self._bounds(model, inputs, cache, size):
                         self._capture_one(model, inputs, cache, workspace, size, bound, side)
+                    if shared_prefix is not None and size > 1:
+                        shared_prefix.update([1] * size, [-1] * size, [])
+                        self._capture_one(model, inputs, cache, workspace, size, None, side,
+                                          shared_prefix, shared_workspace)
         finally:
             side.synchronize()
             # Leave the padding state behind for the first real batch.
@@ -116,7 +126,8 @@ class DecodeGraphs:
                 last = plan
         return sorted(bounds)
 
-    def _capture_one(self, model, inputs, cache, workspace, size, bound, side) -> None:
+    def _capture_one(self, model, inputs, cache, workspace, size, bound, side,
+                     shared_prefix=None, shared_workspace=None) -> None:
         model_input = inputs.view(size, max_context_len=bound)
         params = inputs.sampling_views(size)
         out = self.tokens[:size]
@@ -125,7 +136,9 @@ class DecodeGraphs:
         def step():
             begin_decode(inputs.table, inputs.d["updates"], model_input.input_ids, sources,
                          self.tokens)
-            attention = HipAttention(model_input, cache, decode_workspace=workspace)
+            attention = HipAttention(model_input, cache, decode_workspace=workspace,
+                                     shared_prefix=shared_prefix,
+                                     shared_workspace=shared_workspace)
             hidden = model(model_input.input_ids, model_input.positions, attention=attention)
             logits = model.compute_logits(hidden)
             sample(logits, *params, out=out)
@@ -137,6 +150,9 @@ class DecodeGraphs:
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, pool=self.pool, stream=side):
             logits = step()
+        if shared_prefix is not None:
+            self.shared[size] = (graph, logits, out)
+            return
         self.entries.setdefault(size, []).append((bound, graph, logits, out))
         self.entries[size].sort(key=lambda e: e[0])
 
@@ -163,7 +179,15 @@ class DecodeGraphs:
         graph.replay()
         return logits[:count], tokens[:count]
 
+    def replay_shared(self, count: int, size: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """Replay the graph of ``size`` rows that follows the shared-prefix
+        plan (which holds ``size`` rows, those past ``count`` empty)."""
+        graph, logits, tokens = self.shared[size]
+        graph.replay()
+        return logits[:count], tokens[:count]
+
     def close(self) -> None:
         self.stream.synchronize()
         self.entries.clear()
+        self.shared.clear()
         self.pool = None

@@ -15,8 +15,12 @@ from tinyvllm._validation import _check_positive_int
 from tinyvllm.batch import PreparedBatch
 from tinyvllm.kernels.paged_decode import decode_workspace_bytes
 from tinyvllm.kernels.sampling import resolve_tokens, sample
+from tinyvllm.kernels.shared_prefix import (
+    SharedPrefixPlan, find_shared_prefixes, takes_shared_prefix,
+)
 from tinyvllm.paged_kv import PagedKVCache, resolve_layout
 from tinyvllm.runtime.attention import HipAttention, SDPAAttention, check_backend
+from tinyvllm.runtime.controls import RequestControls
 from tinyvllm.runtime.contracts import (
     ModelInput, MultiQueryMetadata, PagedKVMetadata, SingleQueryMetadata,
 )
@@ -48,6 +52,7 @@ class ModelRunner:
         kv_scales: tuple[float, float] = (1.0, 1.0),
         prefill_graph_tokens: int | None = None,
         kv_cache_layout: str = "auto",
+        shared_prefix_attention: bool = False,
     ) -> None:
         """``kv_cache_dtype``: None keeps K/V in the model dtype;
         ``torch.float8_e4m3fn`` stores them as FP8 E4M3 with ``kv_scales``
@@ -62,13 +67,19 @@ class ModelRunner:
         tokens (and up to 16 items; single-token items of short context only)
         replay captured graphs (0: always eager; None: sized from the model,
         ``default_prefill_graph_tokens``; beyond the reference, which runs
-        these steps eagerly)."""
+        these steps eagerly).
+        ``shared_prefix_attention``: decode steps whose rows share enough cached
+        pages attend over those once for all of them (``SharedPrefixPlan``;
+        beyond the reference, hip backend). Same results up to the order of the
+        softmax's sums; costs one more captured graph per batch size."""
         if prefill_graph_tokens is None:
             prefill_graph_tokens = default_prefill_graph_tokens(model)
         if type(prefill_graph_tokens) is not int or prefill_graph_tokens < 0:
             raise ValueError("prefill_graph_tokens must be a non-negative int")
         if type(enforce_eager) is not bool:
             raise TypeError("enforce_eager must be bool")
+        if type(shared_prefix_attention) is not bool:
+            raise TypeError("shared_prefix_attention must be bool")
         self.model = model.eval()
         self.backend = check_backend(attention_backend, model)
         parameter = next(model.parameters())
@@ -88,6 +99,11 @@ class ModelRunner:
         self.prefill_graphs: PrefillGraphs | None = None
         self.kv_cache: PagedKVCache | None = None
         self.decode_workspace: torch.Tensor | None = None
+        self.shared_prefix: SharedPrefixPlan | None = None
+        self.shared_workspace: torch.Tensor | None = None
+        self._shared_key = self._shared_groups = None
+        self.controls: RequestControls | None = None
+        self.max_num_seqs = max_num_seqs
         # Sampled ids of the last launched step stay here on the device; the
         # next batch's input_token_sources index them (pipelined decode).
         self.sampled = torch.zeros(max_num_seqs, dtype=torch.long, device=self.device)
@@ -120,11 +136,25 @@ class ModelRunner:
                 if ws:
                     self.decode_workspace = torch.empty(ws, dtype=torch.uint8,
                                                         device=self.device)
+                if shared_prefix_attention:
+                    if not takes_shared_prefix(config.num_attention_heads,
+                                               config.num_key_value_heads, config.head_dim):
+                        raise ValueError("shared_prefix_attention needs a head dim that is a "
+                                         "multiple of 8")
+                    self.shared_prefix = SharedPrefixPlan(
+                        num_heads=config.num_attention_heads,
+                        num_kv_heads=config.num_key_value_heads, head_dim=config.head_dim,
+                        block_size=block_size, max_rows=max_num_seqs, device=self.device)
+                    self.shared_workspace = torch.empty(
+                        self.shared_prefix.max_workspace_bytes, dtype=torch.uint8,
+                        device=self.device)
                 if not enforce_eager:
                     self.decode_graphs = DecodeGraphs(self.decode_inputs.stream)
                     self.decode_graphs.capture(model, self.decode_inputs, self.kv_cache,
                                                self.decode_workspace,
-                                               sizes=graph_sizes, tokens=self.sampled)
+                                               sizes=graph_sizes, tokens=self.sampled,
+                                               shared_prefix=self.shared_prefix,
+                                               shared_workspace=self.shared_workspace)
                     # A step writes at most one KV slot per token.
                     graph_tokens = min(prefill_graph_tokens, self.kv_cache.num_slots)
                     if graph_tokens:
@@ -216,6 +246,15 @@ class ModelRunner:
                 or len(batch.sampling_params) != batch.num_samples
                 or any(a >= b for a, b in zip(samples, samples[1:]))):
             raise ValueError("sampling rows must be aligned and ordered")
+        controlled = [p.controlled for p in batch.sampling_params]
+        if any(controlled):
+            histories = batch.sample_histories
+            if histories is None or len(histories) != len(controlled) or any(
+                    c and h is None for c, h in zip(controlled, histories)):
+                raise ValueError("requests with logit controls need their token histories")
+            for params in batch.sampling_params:
+                if any(t >= self.vocab_size for t in params.control_token_ids):
+                    raise ValueError("a logit control names a token out of vocabulary range")
         ends = dict(zip((int(e) - 1 for e in qoff[1:]), batch.request_ids))
         for index, request_id in zip(samples, batch.sample_request_ids):
             if ends.get(index) != request_id:
@@ -287,7 +326,8 @@ class ModelRunner:
     @torch.inference_mode()
     def run_and_sample(self, batch: PreparedBatch,
                        counters) -> tuple[torch.Tensor, torch.Tensor] | None:
-        """(logits, sampled token ids) of the sampled rows, on the device."""
+        """(logits, sampled token ids) of the sampled rows, on the device; the
+        logits after the controls of requests that have any."""
         return self._run(batch, counters=counters, want_tokens=True)
 
     def _run(self, batch, *, counters, want_tokens):
@@ -302,6 +342,8 @@ class ModelRunner:
         if out is None or out[1] is None:
             return out
         logits, tokens = out
+        if batch.sample_histories is not None:
+            tokens = self._sample_controlled(batch, logits, counters)
         rows = tokens.numel()
         if rows <= self.sampled.numel():
             if tokens.data_ptr() != self.sampled.data_ptr():
@@ -310,23 +352,74 @@ class ModelRunner:
             self._prev_count = rows
         return logits, tokens
 
+    def _sample_controlled(self, batch, logits, counters) -> torch.Tensor:
+        """Draw the step's tokens again, behind the requests' controls (a
+        replayed graph has drawn from the logits as they came)."""
+        if self.controls is None:
+            self.controls = RequestControls(max_num_seqs=self.max_num_seqs,
+                                            max_model_len=self.max_model_len,
+                                            vocab_size=self.vocab_size, device=self.device)
+        input_ids, rows = self._step_ids
+        newest = input_ids[:batch.num_samples] if rows is None else input_ids[rows]
+        self.controls.apply(logits, batch, newest.contiguous())
+        return sample_rows(logits, batch.sampling_params, counters)
+
+    def _share(self, batch: PreparedBatch) -> tuple[np.ndarray, np.ndarray] | None:
+        """The batch's groups of rows with a common prefix, where taking it once
+        is worth the step's other kernels."""
+        plan = self.shared_prefix
+        if plan is None or batch.num_items < 2:
+            return None
+        # Tables of one epoch only grow: the groups stay those of the step that
+        # found them.
+        key = (batch.request_ids, batch.kv_table_epochs)
+        if key != self._shared_key or batch.kv_table_epochs is None:
+            self._shared_key = key
+            self._shared_groups = find_shared_prefixes(
+                batch.kv_block_table_ids, batch.kv_block_table_offsets,
+                batch.context_lens_after, batch.kv_block_size)
+        groups, prefixes = self._shared_groups
+        counts = np.bincount(groups[groups >= 0], minlength=len(prefixes))
+        spared = int(((counts - 1) * prefixes).sum()) if len(prefixes) else 0
+        token_bytes = 2 * plan.num_kv_heads * plan.head_dim * self.kv_cache.key.element_size()
+        return (groups, prefixes) if spared * token_bytes >= _SHARED_PREFIX_BYTES else None
+
+    def _plan_shared(self, batch: PreparedBatch, shared, rows: int) -> None:
+        """Plan the step for ``rows`` rows, those past the batch empty."""
+        pad = rows - batch.num_items
+        self.shared_prefix.update(
+            np.pad(np.asarray(batch.context_lens_after, dtype=np.int64), (0, pad)),
+            np.pad(shared[0], (0, pad), constant_values=-1), shared[1])
+
     def _forward(self, batch, counters, want_tokens):
         cache = self.kv_cache
+        self._step_ids = None  # the step's input ids on the device, and the sampled rows
         if self.decode_inputs is not None:
             model_input = self.decode_inputs.prepare(batch, counters)
             if model_input is not None:
-                if self.decode_graphs is not None:  # the graph applies the table updates
-                    replayed = self.decode_graphs.replay(
-                        batch.num_items, max(batch.context_lens_after))
+                self._step_ids = model_input.input_ids, None
+                shared = self._share(batch)
+                if self.decode_graphs is not None:  # the graphs apply the table updates
+                    size = self.decode_graphs.bucket(batch.num_items)
+                    if shared is not None and size in self.decode_graphs.shared:
+                        self._plan_shared(batch, shared, size)
+                        replayed = self.decode_graphs.replay_shared(batch.num_items, size)
+                    else:
+                        replayed = self.decode_graphs.replay(
+                            batch.num_items, max(batch.context_lens_after))
                     if replayed is not None:
                         return replayed
+                if shared is not None:
+                    self._plan_shared(batch, shared, batch.num_items)
                 self.decode_inputs.apply_table_updates()
                 if batch.input_token_sources is not None:
                     resolve_tokens(model_input.input_ids,
                                    self.decode_inputs.d["sources"][:batch.num_items],
                                    self.sampled)
-                attention = HipAttention(model_input, cache,
-                                         decode_workspace=self.decode_workspace)
+                attention = HipAttention(
+                    model_input, cache, decode_workspace=self.decode_workspace,
+                    shared_prefix=None if shared is None else self.shared_prefix,
+                    shared_workspace=self.shared_workspace)
                 hidden = self.model(model_input.input_ids, model_input.positions,
                                     attention=attention)
                 logits = self.model.compute_logits(hidden)
@@ -341,6 +434,8 @@ class ModelRunner:
                 if replayed is not None:
                     logits, tokens = replayed
                     samples = batch.num_samples
+                    d = self.prefill_inputs.d
+                    self._step_ids = d["tokens"], d["sample_rows"][:samples]
                     if samples == 0:
                         return None
                     return logits[:samples], tokens[:samples] if want_tokens else None
@@ -358,11 +453,17 @@ class ModelRunner:
                             attention=self._attention(batch, model_input))
         if batch.num_samples == 0:
             return None
+        self._step_ids = model_input.input_ids, model_input.sample_token_indices
         logits = self.model.compute_logits(hidden, model_input.sample_token_indices)
         tokens = None
         if want_tokens:
             tokens = sample_rows(logits, batch.sampling_params, counters)
         return logits, tokens
+
+    def release(self, request_id: int) -> None:
+        """The request ended: what its controls kept on the device is void."""
+        if self.controls is not None:
+            self.controls.forget(request_id)
 
     def clear(self) -> None:
         try:
@@ -378,9 +479,16 @@ class ModelRunner:
             self.decode_graphs = None
             self.decode_inputs = None
             self.decode_workspace = None
+            self.shared_prefix = self.shared_workspace = None
+            self.controls = None
             self.kv_cache = None
             self.model = None
 
+
+# K and V bytes of a layer that a decode step must spare to attend by a
+# shared-prefix plan: the separate QK-norm + RoPE + KV write and the merge launch
+# cost what reading that much does.
+_SHARED_PREFIX_BYTES = 48 << 20
 
 # GEMM work of an eager prefill step whose launches the host can no longer
 # outrun (~6 ms of dense-layer GEMMs on MI355X, about the host's launch time

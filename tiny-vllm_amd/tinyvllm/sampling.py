@@ -41,6 +41,9 @@ class Sampler:
             raise ValueError("sampling_params must align with logits rows")
         if len(request_ids) != rows:
             raise ValueError("request_ids must align with logits rows")
+        if any(p.controlled for p in sampling_params):
+            raise ValueError("logit controls need the requests' tokens: apply them to the "
+                             "logits first (kernels.logits.apply_logit_controls)")
         if rows == 0:
             return torch.empty((0,), dtype=torch.long, device=logits.device)
         return sample_rows(logits, sampling_params,

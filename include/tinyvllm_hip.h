@@ -416,7 +416,8 @@ int tvllm_argmax(const void* logits, int64_t rows, int64_t vocab,
  * history[slots[r] * capacity + p], p < lengths[r] (at most capacity): i is
  * seen if it stands there, c counts it at p >= prompt_lens[r]. newest, where
  * given, holds the token of position lengths[r] - 1, which the call writes
- * into the history (no other row then reads that slot). Null history: no
+ * into the history (no other row then reads that slot; -1 for an id outside
+ * the vocabulary). Null history: no
  * penalties; null repetition / presence / frequency: 1 / 0 / 0; null newest,
  * bias_offsets, mask_rows: none. A slot outside [0, num_slots), a mask row
  * outside [0, mask_count), ids outside [0, vocab) count as none; bias offsets

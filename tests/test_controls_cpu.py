@@ -68,6 +68,7 @@ def test_entry_point_refuses_wrong_arguments():
             (dict(rows=1 << 40, logits=ptr, out=ptr), b"grid")):
         assert lib.tvllm_logit_controls(*entry_args(**over)) == -1, over
         assert message in lib.tvllm_last_error(), (over, lib.tvllm_last_error())
+    assert lib.tvllm_logit_controls(*entry_args()) == 0 and lib.tvllm_last_error() == b""
 
 
 def test_batches_carry_the_histories_of_controlled_requests():

@@ -121,6 +121,8 @@ def test_update_refuses_wrong_steps():
             plan.update(*step)
     assert (plan.num_rows, plan.num_tasks > 0) == (2, True)
     assert plan.host.equal(before)  # a refused step leaves the plan as it was
+    plan.update([40, 33], [0, 0], [32])
+    assert plan.host.equal(before) and load_kernels().tvllm_last_error() == b""
 
 
 def test_geometries_without_a_kernel_are_refused():
@@ -170,6 +172,8 @@ def test_entry_point_refuses_wrong_arguments():
             (dict(ws=ptr + 4, ws_bytes=64), b"workspace")):
         assert lib.tvllm_paged_decode_shared_prefix(*entry_args(**{**some, **over})) == -1, over
         assert message in lib.tvllm_last_error(), (over, lib.tvllm_last_error())
+    assert lib.tvllm_paged_decode_shared_prefix(*entry_args()) == 0
+    assert lib.tvllm_last_error() == b""
 
 
 def test_planner_entry_point_refuses_small_buffers():
@@ -182,8 +186,8 @@ def test_planner_entry_point_refuses_small_buffers():
     call = lambda n: lib.tvllm_shared_prefix_plan(  # noqa: E731
         one, group, None, 1, 0, 1, 8, 2, 128, 16, buffer, n, ctypes.byref(tasks),
         ctypes.byref(need))
-    assert call(words) == 0 and tasks.value >= 1
     assert call(words - 1) == -1 and b"too small" in lib.tvllm_last_error()
+    assert call(words) == 0 and tasks.value >= 1
     assert lib.tvllm_shared_prefix_plan_words(0, 8, 2) == 0
     assert lib.tvllm_shared_prefix_workspace_size(4, 8, 3, 128) == 0
 

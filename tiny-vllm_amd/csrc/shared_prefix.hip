@@ -516,6 +516,10 @@ shared_prefix_tasks(Args<T> a) {
 #pragma unroll
                 for (int n = 0; n < ND; ++n) o[n] *= alpha;
             }
+            // What follows stays one block: weights worked out in the arms of the
+            // branch above, or put off to the next step, which uses them, would
+            // not run beside the products.
+            asm volatile("" : "+v"(m_run));
             scores(i + 1, next);
             U16x8 pn[2];
             const float m_use = m_run == -INFINITY ? 0.f : m_run - kShift;
@@ -540,6 +544,8 @@ shared_prefix_tasks(Args<T> a) {
             stage(st, i);
             pb[0] = pn[0];
             pb[1] = pn[1];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) asm volatile("" : "+v"(pb[0].w[w]), "+v"(pb[1].w[w]));
             interleave<NC, ND>();
         };
 

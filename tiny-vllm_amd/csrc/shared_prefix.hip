@@ -489,6 +489,13 @@ shared_prefix_tasks(Args<T> a) {
         // The scores of the next tile, the weights of this one and the products
         // of the last one have nothing to wait for in each other, so the matrix
         // cores work while the vector units do.
+        float cm;  // the tile's maximum score of the lane's query, in base-2 units
+        auto maximum = [&](const f32x16& sc) {
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int v = 0; v < 16; ++v) mx[v & 1] = fmaxf(mx[v & 1], sc[v]);
+            return pair_max(fmaxf(mx[0], mx[1])) * a.scale_log2;
+        };
         auto step = [&](Stage& st, int i, f32x16& sc, f32x16& next) {
             __syncthreads();
             trim(st.k, i + 2);
@@ -499,11 +506,8 @@ shared_prefix_tasks(Args<T> a) {
 #pragma unroll
                 for (int v = 0; v < 16; ++v)
                     if (8 * (v >> 2) + 4 * half + (v & 3) >= left) sc[v] = -INFINITY;
+                cm = maximum(sc);
             }
-            float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int v = 0; v < 16; ++v) mx[v & 1] = fmaxf(mx[v & 1], sc[v]);
-            const float cm = pair_max(fmaxf(mx[0], mx[1])) * a.scale_log2;
             const bool grow = cm > m_run + kSlack;  // also: a first finite maximum
             if (i == 0) {  // (nothing to rescale yet)
                 m_run = cm;
@@ -542,10 +546,12 @@ shared_prefix_tasks(Args<T> a) {
             l_run += ps[0] + ps[1];
             values(i - 1);
             stage(st, i);
+            cm = maximum(next);
             pb[0] = pn[0];
             pb[1] = pn[1];
 #pragma unroll
             for (int w = 0; w < 4; ++w) asm volatile("" : "+v"(pb[0].w[w]), "+v"(pb[1].w[w]));
+            asm volatile("" : "+v"(cm));
             interleave<NC, ND>();
         };
 
@@ -588,6 +594,7 @@ shared_prefix_tasks(Args<T> a) {
         }
         __syncthreads();
         scores(0, sa);
+        cm = maximum(sa);
         // Two steps a round, the second past the end where the tiles are odd in
         // number (its weights are 0): a way around it would lead the loop's
         // waits to expect the first one's loads at once.

@@ -60,6 +60,7 @@ template <typename TI, typename TO, bool VEC>
 __global__ void __launch_bounds__(kThreads)
 logit_controls(Args a) {
     __shared__ __align__(16) uint32_t count[kSpan];
+    __shared__ int met[2];
     const int tid = threadIdx.x;
     int64_t bid = blockIdx.x;
     // Block ids are dealt to 8 XCDs in turn: give each a contiguous range.
@@ -133,89 +134,90 @@ logit_controls(Args a) {
     const bool masked = mrow >= 0 && mrow < a.mask_count;
     if (a.in_place && !penal && !biased && !masked) return;
 
-    // A thread reads its tokens' counts where it keeps the tokens themselves.
-    uint32_t c[kPer] = {};
-    uint32_t which[kPer] = {};  // 1 + the token's last entry in the row's biases
+    // Cells that a scan of a list has marked are read by the threads that keep
+    // their tokens, and only if the scan met the span at all.
     auto clear = [&]() {
 #pragma unroll
         for (int i = 0; i < kPer / 4; ++i)
             reinterpret_cast<uint4*>(count)[i * kThreads + tid] = make_uint4(0, 0, 0, 0);
+        if (tid < 2) met[tid] = 0;
         __syncthreads();
     };
-    auto read = [&](uint32_t (&to)[kPer]) {
-        __syncthreads();
+    uint32_t c[kPer];
+    auto read = [&]() {  // whether one of the thread's cells is marked
         if constexpr (VEC) {
 #pragma unroll
             for (int i = 0; i < kPer / 4; ++i) {
                 const uint4 w = *reinterpret_cast<const uint4*>(&count[at(4 * i)]);
-                to[4 * i] = w.x;
-                to[4 * i + 1] = w.y;
-                to[4 * i + 2] = w.z;
-                to[4 * i + 3] = w.w;
+                c[4 * i] = w.x;
+                c[4 * i + 1] = w.y;
+                c[4 * i + 2] = w.z;
+                c[4 * i + 3] = w.w;
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) to[e] = count[at(e)];
+            for (int e = 0; e < kPer; ++e) c[e] = count[at(e)];
         }
+        uint32_t any = 0;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) any |= c[e];
+        return any != 0;
     };
+    bool loaded = !a.in_place;  // else a thread loads what it will change
+    auto need = [&]() {
+        if (!loaded) load();
+        loaded = true;
+    };
+    if (penal || biased) clear();
     if (penal) {
-        clear();
         const uint32_t low = uint32_t(base);
-        const int64_t split = prompt;
-        auto add = [&](int32_t token, int position) {
+        bool found = false;
+        const int split = int(min(max(prompt, int64_t(0)), int64_t(stored)));
+        auto mark = [&](int32_t token, bool in_prompt) {
             const uint32_t i = uint32_t(token) - low;  // (ids below the span wrap past it)
             if (i < uint32_t(kSpan)) {
-                if (position < split) atomicOr(&count[i], kPrompt);
+                found = true;
+                if (in_prompt) atomicOr(&count[i], kPrompt);
                 else atomicAdd(&count[i], 1u);
             }
         };
-        // Several loads of a thread at once, of four ids each where the list's
-        // rows are aligned.
-        constexpr int kAhead = 4;
-        int p = 0;
+        int p = 0;  // where the loop over single ids begins
         if (a.list4) {
+            // Quads of ids, several loads of a thread at once. The quad that the
+            // prompt ends in, and what is left of the list, are single ids of
+            // the first threads.
+            const int quads = stored / 4, mixed = split % 4 ? split / 4 : -1;
+            p = 4 * quads;
             const int4* const list4 = reinterpret_cast<const int4*>(list);
-            for (; p + 4 <= stored; p += 4 * kAhead * kThreads) {
+            constexpr int kAhead = 4;
+            if (mixed >= 0 && mixed < quads && tid < 4)
+                mark(list[4 * mixed + tid], 4 * mixed + tid < split);
+            for (int q0 = 0; q0 < quads; q0 += kAhead * kThreads) {
                 int4 t[kAhead];
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
-                    const int q = p / 4 + k * kThreads + tid;
-                    t[k] = 4 * q + 4 <= stored ? list4[q] : make_int4(-1, -1, -1, -1);
+                    const int q = q0 + k * kThreads + tid;
+                    t[k] = q < quads && q != mixed ? list4[q] : make_int4(-1, -1, -1, -1);
                 }
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
-                    const int q = p + 4 * (k * kThreads + tid);
-                    add(t[k].x, q);
-                    add(t[k].y, q + 1);
-                    add(t[k].z, q + 2);
-                    add(t[k].w, q + 3);
+                    auto four = [&](bool in_prompt) {
+                        mark(t[k].x, in_prompt);
+                        mark(t[k].y, in_prompt);
+                        mark(t[k].z, in_prompt);
+                        mark(t[k].w, in_prompt);
+                    };
+                    if (q0 + k * kThreads + tid < split / 4) four(true);
+                    else four(false);
                 }
             }
-            p = stored & ~3;
         }
-        for (p += tid; p < stored; p += kThreads) add(list[p], p);
-        if (tid == 0 && last >= 0) add(int32_t(last), int(min(n, int64_t(INT32_MAX))));
-        read(c);
-    }
-    if (biased) {
-        __syncthreads();  // the counts are read
-        clear();
-        for (int64_t p = b0 + tid; p < b1; p += kThreads) {
-            const int64_t i = a.bias_tokens[p] - base;
-            if (i >= 0 && i < kSpan) atomicMax(&count[i], uint32_t(p - b0 + 1));
-        }
-        read(which);
-    }
-
-    bool touched = masked;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) touched |= (c[e] | which[e]) != 0u;
-    if (a.in_place) {
-        if (!touched) return;
-        load();
-    }
-    if (touched) {
-        if (penal) {
+        for (p += tid; p < stored; p += kThreads) mark(list[p], p < split);
+        if (tid == 0 && last >= 0) mark(int32_t(last), n < prompt);
+        if (found) met[0] = 1;
+        __syncthreads();
+        if (met[0] && read()) {
+            need();
 #pragma unroll
             for (int e = 0; e < kPer; ++e)
                 if (c[e]) {
@@ -223,34 +225,57 @@ logit_controls(Args a) {
                     const uint32_t times = c[e] & ~kPrompt;
                     x[e] -= freq * float(times);
                     if (times) x[e] -= pres;
+                    if (biased) count[at(e)] = 0;  // the biases find it cleared
                 }
         }
-        if (biased) {
-#pragma unroll
-            for (int e = 0; e < kPer; ++e)
-                if (which[e]) x[e] += a.bias_values[b0 + which[e] - 1];
+    }
+    if (biased) {
+        if (penal) __syncthreads();
+        bool found = false;
+        for (int64_t p = b0 + tid; p < b1; p += kThreads) {
+            const int64_t i = a.bias_tokens[p] - base;
+            if (i >= 0 && i < kSpan) {  // 1 + the token's last entry in the row's list
+                found = true;
+                atomicMax(&count[i], uint32_t(p - b0 + 1));
+            }
         }
-        if (masked) {
-            const uint32_t* const words = a.mask + mrow * a.mask_stride;
-            if constexpr (VEC) {
+        if (found) met[1] = 1;
+        __syncthreads();
+        if (met[1] && read()) {
+            need();
 #pragma unroll
-                for (int g = 0; g < kPer / 8; ++g)
-                    if (at(8 * g) < left) {
-                        const int64_t i = base + at(8 * g);
-                        const uint32_t bits = words[i >> 5] >> (i & 31);  // 8 of one word
+            for (int e = 0; e < kPer; e += 4)
+                if (c[e] | c[e + 1] | c[e + 2] | c[e + 3]) {
+                    float y[4];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (!((bits >> e) & 1u)) x[8 * g + e] = -INFINITY;
-                    }
-            } else {
+                    for (int i = 0; i < 4; ++i) y[i] = a.bias_values[b0 + max(c[e + i], 1u) - 1];
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) {
-                    const int64_t i = base + at(e);
-                    if (at(e) < left && !((words[i >> 5] >> (i & 31)) & 1u)) x[e] = -INFINITY;
+                    for (int i = 0; i < 4; ++i) x[e + i] = c[e + i] ? x[e + i] + y[i] : x[e + i];
                 }
+        }
+    }
+    if (masked) {
+        need();
+        const uint32_t* const words = a.mask + mrow * a.mask_stride;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int g = 0; g < kPer / 8; ++g)
+                if (at(8 * g) < left) {
+                    const int64_t i = base + at(8 * g);
+                    const uint32_t bits = words[i >> 5] >> (i & 31);  // 8 of one word
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (!((bits >> e) & 1u)) x[8 * g + e] = -INFINITY;
+                }
+        } else {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                const int64_t i = base + at(e);
+                if (at(e) < left && !((words[i >> 5] >> (i & 31)) & 1u)) x[e] = -INFINITY;
             }
         }
     }
+    if (!loaded) return;
     if constexpr (VEC) {
 #pragma unroll
         for (int g = 0; g < kPer / 8; ++g) {
@@ -302,7 +327,7 @@ extern "C" int tvllm_logit_controls(
     TVLLM_CHECK(num_slots >= 0 && capacity >= 0 && num_bias >= 0 && num_bias <= INT32_MAX &&
                     mask_count >= 0,
                 "logit_controls: negative sizes");
-    TVLLM_CHECK(capacity <= INT32_MAX, "logit_controls: at most 2^31-1 tokens of history");
+    TVLLM_CHECK(capacity <= INT32_MAX - 65536, "logit_controls: at most 2^31-65537 tokens of history");
     TVLLM_CHECK(!mask_rows || mask_count == 0 || mask_stride >= (vocab + 31) / 32,
                 "logit_controls: a mask row has a bit for every token");
     if (rows == 0) {

@@ -71,6 +71,19 @@ def test_entry_point_refuses_wrong_arguments():
     assert lib.tvllm_logit_controls(*entry_args()) == 0 and lib.tvllm_last_error() == b""
 
 
+def test_entry_point_refuses_outputs_that_overlap_the_logits():
+    lib = load_kernels()
+    ptr = 1 << 20  # fp32 out of bf16 logits of 100 tokens
+    base = dict(rows=4, logits=ptr, dtype=0, out_dtype=2)
+    for stride, out_stride, offset in (
+            (100, 100, 200), (100, 100, -200), (100, 100, 799), (100, 100, -1599),
+            (600, 300, 196), (600, 300, 804)):
+        args = entry_args(**base, stride=stride, out_stride=out_stride, out=ptr + offset)
+        assert lib.tvllm_logit_controls(*args) == -1
+        assert b"not overlap" in lib.tvllm_last_error(), (offset, lib.tvllm_last_error())
+    assert lib.tvllm_logit_controls(*entry_args()) == 0
+
+
 def test_batches_carry_the_histories_of_controlled_requests():
     from tinyvllm.batch import BatchBuilder, StepPlan, WorkItem
     from tinyvllm.request import RequestState, WorkClass

@@ -357,3 +357,43 @@ def test_wrapper_refusals(device):
         with pytest.raises(RuntimeError, match=message):
             apply_logit_controls(**{**dict(logits=x), **args})
     assert apply_logit_controls(x[:0]).shape == (0, 100)
+
+
+@pytest.mark.gpu
+def test_launches_go_to_the_tensors_device(device, monkeypatch):
+    """With another device current, the logits' own is made current for the call."""
+    from tinyvllm.kernels import _extension
+
+    c = make(12, 3, 100)
+    entered = []
+
+    class Recorded(torch.cuda.device):
+        def __init__(self, where):
+            entered.append(where)
+            super().__init__(where)
+
+    monkeypatch.setattr(_extension, "_current_device", lambda: 99)
+    monkeypatch.setattr(torch.cuda, "device", Recorded)
+    out, _ = call(c, device)
+    assert out.device in entered
+    check(out, *formula(c)[:2])
+
+
+@pytest.mark.gpu
+def test_outputs_beside_the_logits_in_one_buffer_or_over_them(device):
+    """Columns of one buffer are apart; rows that overlap others are refused."""
+    from tinyvllm.kernels.logits import apply_logit_controls
+
+    c = make(13, 4, 100)
+    both = torch.zeros(4, 240, device=device)
+    logits, out = both[:, :100], both[:, 120:220]
+    logits.copy_(c["logits"])
+    call(c, device, logits=logits, out=out)
+    check(out, *formula(c)[:2])
+    flat = torch.zeros(1000, device=device)
+    for first, second in ((flat[:400].view(4, 100), flat[100:500].view(4, 100)),
+                          (flat[:400].view(4, 100), flat[60:460].view(4, 100)),
+                          (both[:, :100], both[:, 60:160]), (both[:, 140:240], both[:, 60:160])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            apply_logit_controls(first, out=second)
+    apply_logit_controls(flat[:400].view(4, 100), out=flat[400:800].view(4, 100))

@@ -301,3 +301,71 @@ def test_wrapper_refusals(device):
             call(**over)
     with pytest.raises(RuntimeError, match="match Q shape"):
         call(q=q.transpose(0, 2))
+
+
+def test_launches_go_to_the_tensors_device(device, monkeypatch):
+    """With another device current, the queries' own is made current for the call."""
+    from tinyvllm.kernels import _extension
+
+    b = make_batch(seed=31, heads=8, kv_heads=2, dim=128, dtype=BF16, prefixes=[32],
+                   rows=[(0, 3), (0, 5)])
+    entered = []
+
+    class Recorded(torch.cuda.device):
+        def __init__(self, where):
+            entered.append(where)
+            super().__init__(where)
+
+    args = on_device(b, device)
+    monkeypatch.setattr(_extension, "_current_device", lambda: 99)
+    monkeypatch.setattr(torch.cuda, "device", Recorded)
+    from tinyvllm.kernels.shared_prefix import paged_decode_shared_prefix
+
+    q, cache, meta, plan, out = args
+    paged_decode_shared_prefix(q, cache, 0, meta, plan, out, scale=b["scale"])
+    assert q.device in entered
+    check(b, out)
+
+
+def test_layers_of_a_cache(device):
+    """Every layer by its index, from either end; indexes past them are refused."""
+    from tinyvllm.kernels.shared_prefix import paged_decode_shared_prefix
+    from tinyvllm.paged_kv import PagedKVCache
+
+    for layout in ("token_major", "head_major"):
+        b = make_batch(seed=32, heads=8, kv_heads=2, dim=64, dtype=BF16, prefixes=[48],
+                       rows=[(0, 3), (0, 5), (-1, 20)])
+        q, cache, meta, plan, out = on_device(b, device)
+        deep = PagedKVCache(num_layers=3, num_blocks=b["pool"], block_size=16, num_kv_heads=2,
+                            head_dim=64, device=device, dtype=BF16, layout=layout)
+        for layer in range(3):
+            deep.key[layer].copy_(cache.key[0] * 2 ** layer)
+            deep.value[layer].copy_(cache.value[0] + layer)
+        for layer in (0, 1, 2, -1, -3):
+            n = layer % 3
+            paged_decode_shared_prefix(q, deep, layer, meta, plan, out, scale=b["scale"])
+            check(dict(b, k=deep.key[n].cpu(), v=deep.value[n].cpu()), out)
+        for layer in (3, -4):
+            with pytest.raises(IndexError):
+                paged_decode_shared_prefix(q, deep, layer, meta, plan, out, scale=b["scale"])
+
+
+def test_refused_over_the_queries_and_under_capture(device):
+    """The output over Q is refused; so is an update that a graph would record
+    (its upload would be replayed from a buffer that later updates rewrite)."""
+    from tinyvllm.kernels.shared_prefix import paged_decode_shared_prefix
+
+    b = make_batch(seed=33, heads=8, kv_heads=2, dim=128, dtype=BF16, prefixes=[32],
+                   rows=[(0, 3), (0, 5)])
+    q, cache, meta, plan, out = on_device(b, device)
+    with pytest.raises(RuntimeError, match="output"):
+        paged_decode_shared_prefix(q, cache, 0, meta, plan, q, scale=b["scale"])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out.fill_(0)
+        with pytest.raises(RuntimeError, match="capture"):
+            plan.update(b["lengths"], b["groups"], b["prefixes"])
+    graph.replay()
+    torch.cuda.synchronize()
+    paged_decode_shared_prefix(q, cache, 0, meta, plan, out, scale=b["scale"])
+    check(b, out)

@@ -304,6 +304,18 @@ logit_controls(Args a) {
     }
 }
 
+// Whether `rows` rows of a_width bytes at stride a_stride from a share bytes with
+// rows of b's (columns of one buffer, at one stride, may lie between each other).
+bool rows_overlap(const void* a, int64_t a_stride, int64_t a_width, const void* b,
+                  int64_t b_stride, int64_t b_width, int64_t rows) {
+    const int64_t x = reinterpret_cast<int64_t>(a), y = reinterpret_cast<int64_t>(b);
+    if (x + (rows - 1) * a_stride + a_width <= y || y + (rows - 1) * b_stride + b_width <= x)
+        return false;
+    if (a_stride != b_stride) return true;
+    const int64_t d = ((y - x) % a_stride + a_stride) % a_stride;
+    return d < a_width || d + b_width > a_stride;
+}
+
 }  // namespace
 }  // namespace tvllm
 
@@ -339,8 +351,12 @@ extern "C" int tvllm_logit_controls(
     TVLLM_CHECK(!bias_offsets || num_bias == 0 || (bias_tokens && bias_values),
                 "logit_controls: null pointer");
     TVLLM_CHECK(!mask_rows || mask_count == 0 || mask, "logit_controls: null pointer");
+    const int64_t unit_in = dtype == TVLLM_F32 ? 4 : 2, unit_out = out_dtype == TVLLM_F32 ? 4 : 2;
     TVLLM_CHECK(logits != out || (out_dtype == dtype && out_stride == row_stride),
                 "logit_controls: in place, the output has the logits' type and rows");
+    TVLLM_CHECK(logits == out || !rows_overlap(logits, row_stride * unit_in, vocab * unit_in, out,
+                                               out_stride * unit_out, vocab * unit_out, rows),
+                "logit_controls: the output must be the logits or not overlap them");
     Args a{};
     a.logits = logits;
     a.out = out;

@@ -1272,6 +1272,8 @@ extern "C" int tvllm_paged_decode_shared_prefix(
     TVLLM_CHECK(aligned8(out) && out_token_stride % 4 == 0 && out_head_stride % 4 == 0,
                 "shared_prefix: output rows must be 8-byte aligned");
     TVLLM_CHECK(aligned16(workspace), "shared_prefix: the workspace must be 16-byte aligned");
+    TVLLM_CHECK(q != out, "shared_prefix: the output must not be Q (tasks of a row read Q while "
+                          "others write its output)");
     hipStream_t s = as_hip(stream);
     return dispatch_half(dtype, [&]<int DT>() {
         using T = typename Elem<DT>::T;

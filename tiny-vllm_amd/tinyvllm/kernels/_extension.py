@@ -13,6 +13,7 @@ op raises. Build it with ``python -m tinyvllm.kernels.build``.
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 from functools import lru_cache
 from pathlib import Path
 
@@ -162,6 +163,17 @@ def stream_of(device: torch.device) -> int:
     index = device.index
     return torch._C._cuda_getCurrentRawStream(
         torch.cuda.current_device() if index is None else index)
+
+
+_current_device = torch._C._cuda_getDevice
+_STAY = nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context for a launch on ``device``: its default stream's handle is 0,
+    which names the current device's, so another one is made current for the
+    call. (The usual case, that it is current, costs 0.2 us.)"""
+    return _STAY if _current_device() == device.index else torch.cuda.device(device)
 
 
 def require_gpu(*tensors: torch.Tensor) -> torch.device:

@@ -6,13 +6,23 @@ from __future__ import annotations
 import torch
 
 from tinyvllm.kernels._extension import (
-    check, dtype_code, load_kernels, require_gpu, stream_of,
+    check, dtype_code, load_kernels, on_device, require_gpu, stream_of,
 )
 from tinyvllm.kernels.sampling import _check_logits
 
 
-def _ptr(tensor: torch.Tensor | None) -> int | None:
-    return None if tensor is None else tensor.data_ptr() or None  # (0: empty)
+def _vector(tensor: torch.Tensor | None, dtype: torch.dtype, size: int, index: int,
+            name: str) -> int | None:
+    """Address of a vector of ``size`` (-1: any) elements, None without one."""
+    if tensor is None:
+        return None
+    if (tensor.dtype != dtype or tensor.dim() != 1 or not tensor.is_contiguous()
+            or (tensor.numel() != size and size >= 0)):
+        raise RuntimeError(f"{name} must be a contiguous {dtype} vector"
+                           + ("" if size < 0 else f" of {size}"))
+    if tensor.get_device() != index:
+        raise RuntimeError("tensors must share one GPU device")
+    return tensor.data_ptr() or None  # (0: empty)
 
 
 def apply_logit_controls(
@@ -86,37 +96,38 @@ def apply_logit_controls(
                              or (mask.shape[0] and mask.shape[1] < -(-vocab // 32))):
         raise RuntimeError("mask must be int32 [masks, words] with unit last stride and a bit "
                            "for every token")
-    for tensor in (history, mask):
-        if tensor is not None and tensor.get_device() != index:
+    history_ptr = mask_ptr = None
+    num_slots = capacity = masks = mask_stride = num_bias = 0
+    if history is not None:
+        if history.get_device() != index:
             raise RuntimeError("tensors must share one GPU device")
-    for names, dtype, size, tensors in (
-            (("repetition", "presence", "frequency"), torch.float32, rows,
-             (repetition, presence, frequency)),
-            (("slots", "lengths", "prompt_lens", "newest", "mask_rows"), torch.long, rows,
-             (slots, lengths, prompt_lens, newest, mask_rows)),
-            (("bias_offsets",), torch.long, rows + 1, (bias_offsets,)),
-            (("bias_tokens",), torch.int32, None, (bias_tokens,)),
-            (("bias_values",), torch.float32, None, (bias_values,))):
-        for name, tensor in zip(names, tensors):
-            if tensor is None:
-                continue
-            shape = tensor.shape
-            if tensor.dtype != dtype or len(shape) != 1 or not tensor.is_contiguous() or (
-                    size is not None and shape[0] != size):
-                raise RuntimeError(f"{name} must be a contiguous {dtype} vector"
-                                   + ("" if size is None else f" of {size}"))
-            if tensor.get_device() != index:
-                raise RuntimeError("tensors must share one GPU device")
+        num_slots, capacity = history.shape
+        history_ptr = history.data_ptr() or None
+    if mask is not None:
+        if mask.get_device() != index:
+            raise RuntimeError("tensors must share one GPU device")
+        masks, mask_stride, mask_ptr = mask.shape[0], mask.stride(0), mask.data_ptr() or None
+    if bias_tokens is not None:
+        num_bias = bias_values.numel()
+    f32, i64 = torch.float32, torch.long
+    args = (
+        _vector(repetition, f32, rows, index, "repetition"),
+        _vector(presence, f32, rows, index, "presence"),
+        _vector(frequency, f32, rows, index, "frequency"),
+        history_ptr, num_slots, capacity,
+        _vector(slots, i64, rows, index, "slots"),
+        _vector(lengths, i64, rows, index, "lengths"),
+        _vector(prompt_lens, i64, rows, index, "prompt_lens"),
+        _vector(newest, i64, rows, index, "newest"),
+        _vector(bias_tokens, torch.int32, num_bias, index, "bias_tokens"),
+        _vector(bias_values, f32, -1, index, "bias_values"),
+        _vector(bias_offsets, i64, rows + 1, index, "bias_offsets"), num_bias,
+        mask_ptr, masks, mask_stride, _vector(mask_rows, i64, rows, index, "mask_rows"))
     if rows == 0:
         return out
-    check(load_kernels().tvllm_logit_controls(
-        logits.data_ptr(), rows, vocab, logits.stride(0), _ptr(repetition), _ptr(presence),
-        _ptr(frequency), _ptr(history), 0 if history is None else history.shape[0],
-        0 if history is None else history.shape[1], _ptr(slots), _ptr(lengths),
-        _ptr(prompt_lens), _ptr(newest), _ptr(bias_tokens), _ptr(bias_values),
-        _ptr(bias_offsets), 0 if bias_tokens is None else bias_tokens.numel(), _ptr(mask),
-        0 if mask is None else mask.shape[0], 0 if mask is None else mask.stride(0),
-        _ptr(mask_rows), out.data_ptr(), out.stride(0), dtype_code(logits.dtype),
-        dtype_code(out.dtype), stream_of(device),
-    ))
+    with on_device(device):
+        check(load_kernels().tvllm_logit_controls(
+            logits.data_ptr(), rows, vocab, logits.stride(0), *args, out.data_ptr(),
+            out.stride(0), dtype_code(logits.dtype), dtype_code(out.dtype), stream_of(device),
+        ))
     return out

@@ -11,13 +11,14 @@ import torch
 
 from tinyvllm._validation import _check_positive_int
 from tinyvllm.kernels._extension import (
-    cache_format, check, dtype_code, load_kernels, require_gpu, stream_of,
+    cache_format, check, dtype_code, load_kernels, on_device, require_gpu, stream_of,
 )
 from tinyvllm.paged_kv import PagedKVCache
 from tinyvllm.runtime.contracts import SingleQueryMetadata
 
 _HEADER = 16     # words of a plan ahead of its lists
 _TASK_WORDS = 8
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 def takes_shared_prefix(num_heads: int, num_kv_heads: int, head_dim: int) -> bool:
@@ -34,7 +35,7 @@ class SharedPrefixPlan:
     call replays over whatever plan was last uploaded, as long as that has the
     captured number of rows. Its upload is ordered on the current stream: calls
     by the old plan on other streams must be done, and calls by the new one
-    there must wait for it."""
+    there must wait for it. It is refused under graph capture."""
 
     def __init__(self, *, num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
                  max_rows: int, device: torch.device | str) -> None:
@@ -75,6 +76,8 @@ class SharedPrefixPlan:
             raise ValueError("context_lens and row_groups must be vectors of one length")
         if len(lengths) > self.max_rows:
             raise ValueError("more rows than the plan holds")
+        if self._uploaded is not None and _capturing():
+            raise RuntimeError("a plan cannot be updated under graph capture")
         if self._pending:  # stream order does not hold back the CPU's writes
             self._uploaded.synchronize()
             self._pending = False
@@ -141,52 +144,62 @@ def paged_decode_shared_prefix(
     share are read and multiplied once for all of them.
 
     The context lengths are those of ``plan.update`` (``metadata.context_lens``
-    is not read). ``workspace`` (optional, uint8, 16-byte aligned): at least
+    is not read); ``output`` is memory of its own, and no row of it is listed
+    twice. ``workspace`` (optional, uint8, 16-byte aligned): at least
     ``plan.workspace_bytes``, under capture ``plan.max_workspace_bytes``; when
     omitted it is allocated from torch's caching allocator (inside graph
     capture that is the graph's private pool)."""
-    lib = load_kernels()
-    k, v = cache.key[layer_idx], cache.value[layer_idx]
+    key, value, layers = cache.key, cache.value, cache.num_layers
     rows, blocks = metadata.query_rows, metadata.block_table_ids
-    offsets = metadata.block_table_offsets
-    device = require_gpu(q, k, v, output, rows, blocks, offsets, plan.data)
+    offsets, data = metadata.block_table_offsets, plan.data
+    if not -layers <= layer_idx < layers:
+        raise IndexError("layer_idx is not a layer of the cache")
+    device = require_gpu(q, key, value, output, rows, blocks, offsets, data)
     if q.dim() != 3:
         raise RuntimeError("Q must be a GPU [tokens, heads, dim] tensor")
-    if k.stride() != v.stride():
+    strides = key.stride()
+    if strides != value.stride():
         raise RuntimeError("K/V caches must share one layout")
-    if q.dtype not in (torch.float16, torch.bfloat16):
+    dtype = q.dtype
+    if dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("Q must use float16 or bfloat16")
-    if (k.dtype != q.dtype and not cache.fp8) or output.dtype != q.dtype:
+    if (key.dtype != dtype and not cache.fp8) or output.dtype != dtype:
         raise RuntimeError("Q/K/V/output must share device and dtype")
-    if output.shape != q.shape or q.stride(2) != 1 or output.stride(2) != 1:
+    q_token, q_head, q_dim = q.stride()
+    if output.shape != q.shape or q_dim != 1 or output.stride(2) != 1:
         raise RuntimeError("output must match Q shape with unit last stride")
     for tensor in (rows, blocks, offsets):
         if tensor.dtype != torch.long or tensor.dim() != 1 or not tensor.is_contiguous():
             raise RuntimeError("metadata must be contiguous GPU int64 vectors on Q's device")
-    if offsets.numel() != rows.numel() + 1:
+    num_rows = rows.numel()
+    if offsets.numel() != num_rows + 1:
         raise RuntimeError("metadata lengths must align")
+    _, heads, dim = q.shape
     if (plan.num_heads, plan.num_kv_heads, plan.head_dim, plan.block_size) != (
-            q.shape[1], cache.num_kv_heads, q.shape[2], cache.block_size):
+            heads, cache.num_kv_heads, dim, cache.block_size):
         raise RuntimeError("the plan was made for another geometry")
-    if plan.num_rows != rows.numel():
+    if plan.num_rows != num_rows:
         raise RuntimeError("the plan was made for another number of rows")
-    if plan.num_rows == 0:
+    if num_rows == 0:
         return
-    # A captured call is replayed over later plans: it takes the bounds.
-    if torch.cuda.is_current_stream_capturing():
-        tasks, need = plan.max_tasks, plan.max_workspace_bytes
-    else:
-        tasks, need = plan.num_tasks, plan.workspace_bytes
-    if workspace is None or workspace.numel() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    elif require_gpu(q, workspace) != device or workspace.dtype != torch.uint8 \
-            or not workspace.is_contiguous():
-        raise RuntimeError("workspace must be contiguous uint8 on Q's device")
-    check(lib.tvllm_paged_decode_shared_prefix(
-        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(), output.data_ptr(),
-        output.stride(0), output.stride(1), rows.data_ptr(), blocks.data_ptr(),
-        offsets.data_ptr(), plan.data.data_ptr(), plan.num_rows, plan.max_rows, tasks,
-        plan.num_heads, plan.num_kv_heads, plan.head_dim, cache.num_slots, k.stride(0),
-        k.stride(1), cache.block_size, float(scale), workspace.data_ptr() if need else None,
-        need, dtype_code(q.dtype), *cache_format(cache), stream_of(device),
-    ))
+    with on_device(device):
+        # A captured call is replayed over later plans: it takes the bounds.
+        if _capturing():
+            tasks, need = plan.max_tasks, plan.max_workspace_bytes
+        else:
+            tasks, need = plan.num_tasks, plan.workspace_bytes
+        if workspace is None or workspace.numel() < need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        elif require_gpu(q, workspace) != device or workspace.dtype != torch.uint8 \
+                or not workspace.is_contiguous():
+            raise RuntimeError("workspace must be contiguous uint8 on Q's device")
+        # Addresses of the layer, without views of it (1.2 us each).
+        skip = layer_idx % layers * strides[0] * key.element_size()
+        check(load_kernels().tvllm_paged_decode_shared_prefix(
+            q.data_ptr(), q_token, q_head, key.data_ptr() + skip, value.data_ptr() + skip,
+            output.data_ptr(), output.stride(0), output.stride(1), rows.data_ptr(),
+            blocks.data_ptr(), offsets.data_ptr(), data.data_ptr(), num_rows, plan.max_rows,
+            tasks, heads, plan.num_kv_heads, dim, cache.num_slots, strides[1], strides[2],
+            cache.block_size, float(scale), workspace.data_ptr() if need else None, need,
+            dtype_code(dtype), *cache_format(cache), stream_of(device),
+        ))

@@ -382,7 +382,8 @@ class ModelRunner:
         counts = np.bincount(groups[groups >= 0], minlength=len(prefixes))
         spared = int(((counts - 1) * prefixes).sum()) if len(prefixes) else 0
         token_bytes = 2 * plan.num_kv_heads * plan.head_dim * self.kv_cache.key.element_size()
-        return (groups, prefixes) if spared * token_bytes >= _SHARED_PREFIX_BYTES else None
+        least = _SHARED_PREFIX_BYTES * (1 + batch.num_items / _SHARED_PREFIX_ROWS)
+        return (groups, prefixes) if spared * token_bytes >= least else None
 
     def _plan_shared(self, batch: PreparedBatch, shared, rows: int) -> None:
         """Plan the step for ``rows`` rows, those past the batch empty."""
@@ -486,9 +487,16 @@ class ModelRunner:
 
 
 # K and V bytes of a layer that a decode step must spare to attend by a
-# shared-prefix plan: the separate QK-norm + RoPE + KV write and the merge launch
-# cost what reading that much does.
-_SHARED_PREFIX_BYTES = 48 << 20
+# shared-prefix plan, and the rows that double them: the separate QK-norm + RoPE
+# + KV write and the merge launch cost what reading that much does, more with
+# more rows. A decode step per layer, plain -> shared, with MiB spared:
+#   Qwen3-0.6B   2 rows:  64: 55.6 -> 56.3 us   123: 67.8 -> 64.2
+#                8 rows:  56: 48.0 -> 49.0      112: 52.9 -> 51.0
+#   Qwen3-8B    32 rows:  62: 155.4 -> 159.3    124: 162.0 -> 159.5
+#               64 rows: 126: 174.7 -> 177.9    252: 187.4 -> 178.3
+# and 64 rows behind 2048 shared tokens (504 MiB): 213.5 -> 178.5.
+_SHARED_PREFIX_BYTES = 72 << 20
+_SHARED_PREFIX_ROWS = 50
 
 # GEMM work of an eager prefill step whose launches the host can no longer
 # outrun (~6 ms of dense-layer GEMMs on MI355X, about the host's launch time

@@ -125,6 +125,37 @@ struct Args {
     int64_t entries;   // room in the two
 };
 
+// Asks for the 64-byte lines that the arguments lie in, all at once.
+template <typename T>
+__device__ __forceinline__ void touch(const Args<T>& a) {
+    asm volatile("" ::"s"(a.q), "s"(a.plan), "s"(a.entries));
+}
+
+// The plan's header, in one load, and whether the call is what it was made for.
+struct PlanHead {
+    int32_t w[8];
+    template <typename T>
+    __device__ bool fits(const Args<T>& a) const {
+        return (w[H_ROWS] == a.num_rows) & (w[H_HEADS] == a.heads) &
+               (w[H_KV_HEADS] == a.kv_heads) & (w[H_DIM] == a.head_dim) &
+               (w[H_BLOCK] == a.block_size) & (w[H_PARTS] <= a.entries);
+    }
+};
+__device__ __forceinline__ PlanHead load_head(const int32_t* plan) {
+    PlanHead h;
+    const int4 lo = *reinterpret_cast<const int4*>(plan);
+    const int4 hi = *reinterpret_cast<const int4*>(plan + 4);
+    h.w[0] = lo.x;
+    h.w[1] = lo.y;
+    h.w[2] = lo.z;
+    h.w[3] = lo.w;
+    h.w[4] = hi.x;
+    h.w[5] = hi.y;
+    h.w[6] = hi.z;
+    h.w[7] = hi.w;
+    return h;
+}
+
 template <int I, int N, typename F>
 __device__ __forceinline__ void static_for(F&& f) {
     if constexpr (I < N) {
@@ -277,21 +308,25 @@ shared_prefix_tasks(Args<T> a) {
     constexpr int kTileBytes = 2 * 2 * (K_TILE + V_TILE);
     constexpr int kMergeBytes = 4 * kNarrow * (4 * DP + 8);
     __shared__ __align__(16) char lds[kTileBytes > kMergeBytes ? kTileBytes : kMergeBytes];
+    __shared__ int2 spots[kWide];
 
+    // A chain of loads leads to the keys: the plan's header and the task, the
+    // row's offset, its pages, their rows. What can goes out together (the plan
+    // holds max_tasks tasks whatever the header says).
     const int32_t* const plan = a.plan;
-    if (int(blockIdx.x) >= plan[H_TASKS] || plan[H_ROWS] != a.num_rows ||
-        plan[H_HEADS] != a.heads || plan[H_KV_HEADS] != a.kv_heads ||
-        plan[H_DIM] != a.head_dim || plan[H_BLOCK] != a.block_size ||
-        plan[H_PARTS] > a.entries)
-        return;
     const int32_t* const task = plan + a.tasks_at + int64_t(blockIdx.x) * kTaskWords;
-    const int32_t* const members = plan + a.members_at + task[T_MEMBER];
-    const int q_begin = (task[T_QUERIES] >> 8) * kNarrow, q_count = task[T_QUERIES] & 0xff;
-    const int kvh = task[T_KVH];
-    const int k0 = task[T_K0], k1 = task[T_K1], part = task[T_PART];
+    const int t_member = task[T_MEMBER], t_queries = task[T_QUERIES], kvh = task[T_KVH];
+    const int t_heads = task[T_HEADS], k0 = task[T_K0], k1 = task[T_K1];
+    const int part = task[T_PART], t_row = task[T_ROW];
+    const PlanHead head = load_head(plan);
+    asm volatile("" ::"s"(t_member), "s"(t_queries), "s"(kvh), "s"(t_heads), "s"(k0), "s"(k1),
+                 "s"(part), "s"(t_row), "s"(head.w[0]), "s"(head.w[7]));
+    if (int(blockIdx.x) >= head.w[H_TASKS] || !head.fits(a)) return;
+    const int32_t* const members = plan + a.members_at + t_member;
+    const int q_begin = (t_queries >> 8) * kNarrow, q_count = t_queries & 0xff;
     const int D = a.head_dim;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int64_t table = a.offsets[task[T_ROW]];
+    const int64_t table = a.offsets[t_row];
     const uint32_t* const ids = reinterpret_cast<const uint32_t*>(a.blocks + table);
     const uint32_t row_bytes = uint32_t(a.css * EB);
     const char* const kbase = static_cast<const char*>(a.k) + int64_t(kvh) * a.chs * EB;
@@ -307,11 +342,14 @@ shared_prefix_tasks(Args<T> a) {
         row = members[g];
         head = (kvh + x) * a.group + (q_begin + i - g * a.group);
     };
-    // Where a row's part goes; rows of one part are written to the output.
-    auto entry_of = [&](int row, int head, bool& direct) -> int64_t {
-        const int first = plan[a.rows_at + 2 * row];
-        direct = plan[a.rows_at + 2 * row + 1] == 1;
-        return (int64_t(first) + part) * a.heads + head;
+    // Where a row's part goes: (first part, parts) of the row, looked up ahead
+    // and kept in LDS. Rows of one part are written to the output.
+    auto spot_of = [&](int row) {
+        return *reinterpret_cast<const int2*>(plan + a.rows_at + 2 * row);
+    };
+    auto entry_of = [&](int2 spot, int head, bool& direct) -> int64_t {
+        direct = spot.y == 1;
+        return (int64_t(spot.x) + part) * a.heads + head;
     };
 
     // ------------------------------------------------------------- wide --
@@ -332,19 +370,7 @@ shared_prefix_tasks(Args<T> a) {
         // Waves past the queries take the last one along: a second path through
         // the loop for them would make the others wait for its loads.
         const int qi = wave * 32 + col;
-        int row, head;
-        query(min(qi, q_count - 1), 0, row, head);
-
         U16x8 qv[NC];
-        {
-            const T* qrow = a.q + a.rows[row] * a.qts + head * a.qhs;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const int d = 16 * c + 8 * half;
-                qv[c] = d < D ? *reinterpret_cast<const U16x8*>(qrow + d) : U16x8{};
-            }
-        }
-
         const int ntiles = (k1 - k0 + BK - 1) / BK;
         const uint32_t last = uint32_t(k1 - 1);
         // Staging: LPR lanes side by side load a row's whole 128-byte lines
@@ -569,6 +595,11 @@ shared_prefix_tasks(Args<T> a) {
             load_ids(id2, 2);
             load_ids(id3, 3);
             load_ids(id, 4);
+            int row, head;
+            query(min(qi, q_count - 1), 0, row, head);
+            keep_order();
+            const int64_t qtoken = a.rows[row];
+            const int2 spot = spot_of(row);
             locate(off0, id0, 0);
             locate(off1, id1, 1);
             locate(st0.off, id2, 2);
@@ -576,6 +607,13 @@ shared_prefix_tasks(Args<T> a) {
             keep_order();
             load(first, off0, kbase);
             load(second, off1, kbase);
+            keep_order();
+            const T* const qrow = a.q + qtoken * a.qts + head * a.qhs;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int d = 16 * c + 8 * half;
+                qv[c] = d < D ? *reinterpret_cast<const U16x8*>(qrow + d) : U16x8{};
+            }
             keep_order();
             load(st0.v, off0, vbase);
             load(st0.k, st0.off, kbase);
@@ -587,6 +625,7 @@ shared_prefix_tasks(Args<T> a) {
             // of 0: zeros, as LDS may hold NaNs.
             for (int x = tid; x < V_TILE / 8; x += kThreads)
                 reinterpret_cast<U16x8*>(vs + V_TILE)[x] = U16x8{};
+            if (half == 0) spots[qi] = spot;
             trim(first, 0);
             store_k(first, 0);
             trim(second, 1);
@@ -603,8 +642,6 @@ shared_prefix_tasks(Args<T> a) {
             step(st0, i, sa, sb);
             step(st1, i + 1, sb, sa);
         }
-        bool direct;
-        const int64_t entry = entry_of(row, head, direct);
         __syncthreads();  // V of the last tile
         values(steps - 1);
 
@@ -621,6 +658,10 @@ shared_prefix_tasks(Args<T> a) {
         if (__syncthreads_or(again)) return true;
         const float l = pair_sum(l_run);
         if (qi >= q_count) return false;
+        int row, head;
+        query(qi, 0, row, head);
+        bool direct;
+        const int64_t entry = entry_of(spots[qi], head, direct);
         if (direct) {
             const float inv = a.v_scale / l;
             T* orow = a.out + a.rows[row] * a.ots + head * a.ohs + 4 * half;
@@ -672,10 +713,11 @@ shared_prefix_tasks(Args<T> a) {
         float m_run = -INFINITY, l_run = 0.f;
 
         // The waves of a head take its keys in equal, consecutive shares.
-        const int heads = task[T_HEADS], shares = 4 / heads;
+        const int heads = t_heads, shares = 4 / heads;
         const int x = wave / shares;  // this wave's KV head, of the task's
         const char* const kbase = static_cast<const char*>(a.k) + int64_t(kvh + x) * a.chs * EB;
         const char* const vbase = static_cast<const char*>(a.v) + int64_t(kvh + x) * a.chs * EB;
+        int2 spot;  // wave 0, which always has keys: where its lanes' results go
         const int per = ((k1 - k0 + shares - 1) / shares + 15) & ~15;
         const int t_begin = k0 + (wave - x * shares) * per, t_end = min(k1, t_begin + per);
         if (t_begin < t_end) {
@@ -725,6 +767,11 @@ shared_prefix_tasks(Args<T> a) {
             {
                 int row, head;
                 query(q0 + min(col, qn - 1), x, row, head);
+                if (wave == 0 && lane < heads * qn) {
+                    int r, h;
+                    query(q0 + lane % qn, 0, r, h);
+                    spot = spot_of(r);
+                }
                 const T* qrow = a.q + a.rows[row] * a.qts + head * a.qhs;
 #pragma unroll
                 for (int c = 0; c < KS; ++c) {
@@ -856,6 +903,7 @@ shared_prefix_tasks(Args<T> a) {
         float2* const sml = reinterpret_cast<float2*>(so + 4 * kNarrow * DP);  // [4][16]
         __syncthreads();  // a repeated call: the last one's reads are done
         if (quad == 0) sml[wave * kNarrow + col] = make_float2(m_run, l_run);
+        if (wave == 0 && lane < heads * qn) spots[lane] = spot;
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
             const int h = 4 * quad + v;
@@ -892,7 +940,7 @@ shared_prefix_tasks(Args<T> a) {
             int row, head;
             query(q0 + h, y, row, head);
             bool direct;
-            const int64_t entry = entry_of(row, head, direct);
+            const int64_t entry = entry_of(spots[y * qn + h], head, direct);
             if (direct) {
                 const float inv = a.v_scale / l;
                 uint2 w;
@@ -919,18 +967,22 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads)
 shared_prefix_merge(Args<T> a) {
     constexpr int LPH = DP / 4, PAR = 64 / LPH, B = 8;
-    const int32_t* const plan = a.plan;
-    if (plan[H_ROWS] != a.num_rows || plan[H_HEADS] != a.heads || plan[H_DIM] != a.head_dim ||
-        plan[H_PARTS] > a.entries)
-        return;
-    const int64_t item = int64_t(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
-    if (item >= int64_t(a.num_rows) * a.heads) return;
-    const int r = int(item / a.heads), h = int(item - int64_t(r) * a.heads);
+    touch(a);
+    const uint32_t item = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+    if (item >= uint32_t(a.num_rows) * uint32_t(a.heads)) return;
+    const int r = int(item / uint32_t(a.heads)), h = int(item - uint32_t(r) * uint32_t(a.heads));
     const int lane = threadIdx.x & 63, sub = lane / LPH, d = 4 * (lane % LPH);
-    const int parts = plan[a.rows_at + 2 * r + 1];
+    // The row's parts and its output row are asked for along with the header.
+    const int32_t* const plan = a.plan;
+    const int2 spot = *reinterpret_cast<const int2*>(plan + a.rows_at + 2 * r);
+    const int64_t out_row = a.rows[r];
+    const PlanHead head = load_head(plan);
+    asm volatile("" ::"v"(spot.x), "v"(spot.y), "v"(out_row), "s"(head.w[0]), "s"(head.w[7]));
+    if (!head.fits(a)) return;
+    const int parts = spot.y;
     if (parts == 1) return;
     const bool has = d < a.head_dim;
-    const int64_t first = int64_t(plan[a.rows_at + 2 * r]) * a.heads + h;
+    const int64_t first = int64_t(spot.x) * a.heads + h;
     const float2* const pml = a.part_ml + first;
     const float* const po = a.part_o + first * a.head_dim + (has ? d : 0);
     const int64_t step = int64_t(a.heads) * a.head_dim;
@@ -983,7 +1035,7 @@ shared_prefix_merge(Args<T> a) {
     uint2 w;
     w.x = pack2<T>(sum.x * inv, sum.y * inv);
     w.y = pack2<T>(sum.z * inv, sum.w * inv);
-    *reinterpret_cast<uint2*>(a.out + a.rows[r] * a.ots + h * a.ohs + d) = w;
+    *reinterpret_cast<uint2*>(a.out + out_row * a.ots + h * a.ohs + d) = w;
 }
 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -1271,6 +1323,7 @@ extern "C" int tvllm_paged_decode_shared_prefix(
                 "shared_prefix: Q rows must be 16-byte aligned");
     TVLLM_CHECK(aligned8(out) && out_token_stride % 4 == 0 && out_head_stride % 4 == 0,
                 "shared_prefix: output rows must be 8-byte aligned");
+    TVLLM_CHECK(aligned16(plan), "shared_prefix: the plan must be 16-byte aligned");
     TVLLM_CHECK(aligned16(workspace), "shared_prefix: the workspace must be 16-byte aligned");
     TVLLM_CHECK(q != out, "shared_prefix: the output must not be Q (tasks of a row read Q while "
                           "others write its output)");

@@ -241,7 +241,8 @@ int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* groups,
  * geometry and block_size are those it was made with, or nothing is written):
  * q, out, caches, rows, blocks and offsets as there; the context lengths are
  * the plan's. head_dim a multiple of 8 up to 256; cache rows in aligned
- * 8-element units, q rows 16-byte aligned, out rows 8-byte. workspace (16-byte
+ * 8-element units, q rows and the plan 16-byte aligned, out rows 8-byte; out
+ * is not q's memory. workspace (16-byte
  * aligned, no initialisation) holds the partial results of this call; calls
  * that may overlap need their own. fp32 softmax and sums; the weights enter
  * the products as two 16-bit terms of the cache's type, or, over keys shared by

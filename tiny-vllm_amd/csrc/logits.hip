@@ -12,12 +12,21 @@
 // sampler takes the logits as they are: tinyvllm/sampling.py:21-72).
 //
 // MI355X design: one pass over the vocabulary, a workgroup per row and span of
-// 8192 tokens, 8 to a thread. The history is a list of token ids by position
+// 8192 tokens, 16 to a thread. The history is a list of token ids by position
 // (what a decode step can append to on the device, where the newest token
 // still is when the next step starts); each workgroup scans its row's list and
 // counts the ids of its own span in LDS, so no table of counts per request and
 // token has to be kept, cleared or read. The spans of a row sit on one XCD, so
 // its L2 serves the list to all but the first.
+//
+// Measured on one MI355X (kernel trace), 151936 tokens: 256 rows fp32, lists of
+// 2048-32768 ids, biases and masks 102 us, 3.3 TB/s of logits in and out and
+// lists; 64 rows bf16, lists up to 4096 15.5 us; one row 6.2 us. The first is
+// bound by the scans: without controls it takes 71 us (torch's copy 59), with
+// lists of at most 8192 ids 83, every span's workgroup looking at every id.
+// Threads and tokens per thread, us for the first two: 512 x 16 107 / 15.6
+// (when chosen), 512 x 8 134 / 20.7, 1024 x 8 147 / 25.0, 256 x 16 119 / 15.0,
+// 1024 x 16 117 / 19.2, 512 x 32 110 / 17.0.
 #include "common.h"
 
 #include <type_traits>

@@ -20,14 +20,36 @@
 //    of 256 CUs) where the keys allow. One launch runs them all, so the
 //    compute-bound shared part and the memory-bound own parts overlap; a
 //    second merges the parts of each (row, head).
-//  * Wide tasks (above 16 query vectors): K/V tiles of 64 tokens in LDS, 32
+//  * Wide tasks (above 16 query vectors): K/V tiles of 32 tokens in LDS, 32
 //    queries per wave on the 32x32x16 MFMA: S^T = K Q^T leaves a lane with 16
 //    tokens of its own query, which are the k values of its column in O^T +=
 //    V^T P^T, so P never moves. V is read from LDS through the transposing
-//    load, so it is staged as it lies in the cache.
+//    load, so it is staged as it lies in the cache. A step multiplies the next
+//    tile's scores, works out this tile's weights and multiplies the last
+//    tile's values: three chains that do not wait for each other, their
+//    instructions interleaved one matrix instruction at a time (without that
+//    order a step takes 1.29 times as long).
 //  * Narrow tasks (up to 16 query vectors; a row's own keys at GQA groups up
 //    to 16): each of four waves streams its quarter of the keys straight into
-//    registers, Q.K^T and P.V on 16-wide MFMAs, and the waves merge in LDS.
+//    registers (or the waves take the KV heads of a short range), Q.K^T and P.V
+//    on 16-wide MFMAs, and the waves merge in LDS.
+//
+// Measured on one MI355X (kernel trace; tasks + merge, bf16 and 32 / 8 heads of
+// 128 if not said otherwise):
+//   64 rows behind 2048 shared tokens, 64-512 own           23.5 + 4.1 us
+//   256 rows behind 32768, 1-1024 own                        220 + 10.5 us
+//   16 rows behind 32768, 64 / 8 heads, FP8 cache             35 + 8.2 us
+//   own keys alone, 256 rows of 2048         6.3 TB/s (5.2 TB/s from FP8)
+// What bounds them: the wide path's step, 32 tokens by 2 x 128 queries in
+// 1.24 us on a CU, about 830 TFLOP/s over the card where a large matrix product
+// reaches 1375. No unit is full (matrix 34 %, vector 42 %, LDS 27 % busy); left
+// out one at a time, staging is 21 % of it, the products with V 23 %, with K
+// 17 %, the loads 9 %, the exponentials 3 %. Short calls are bound by chains of
+// dependent loads (plan, page, row) and by the second launch.
+// 64 queries per wave at one workgroup per CU halve the staging and were
+// slower (one wave per SIMD has nothing to run while it waits); so were narrow
+// tasks ahead of the wide ones or between them (64 rows behind 2048: 26.2 and
+// 26.6 us; 256 behind 32768: 284 and 294).
 #include "common.h"
 
 #include <algorithm>
@@ -42,7 +64,11 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kThreads = 256;
 constexpr int kWide = 128;    // query vectors of a wide task (32 per wave)
-constexpr int kNarrow = 16;   // query vectors of a narrow one
+// Query vectors of a narrow one: one 16-wide matrix instruction takes them. A
+// second pass over the keys costs more than a wide task with idle columns: 20
+// vectors a KV head, 8 heads behind 4096 keys 9.6 us wide, 13.2 narrow; 32 of
+// them behind 32768 31.5 and 47.7; 64 33.3 and 90.2.
+constexpr int kNarrow = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 // Running maxima of the wide path rise only when a tile's maximum exceeds them
 // by more than this (log2 units), so most tiles skip the rescale.
@@ -71,7 +97,9 @@ constexpr int64_t kMaxParts = 64;   // splits of one unit
 constexpr int64_t kMaxContext = INT32_MAX - 4096;  // token numbers past a tile's end fit in 32 bits
 constexpr int64_t kMaxSplits = 1024;  // tasks that splitting adds, all units together
 // What a task costs beside its keys (its chain of first loads, the merge in LDS
-// and the write of its part), in keys.
+// and the write of its part), in keys. At 32 / 128 / 512: 64 rows behind 2048
+// 24.3 / 23.7 / 24.1 us, 49 rows in 6 groups 41.6 / 38.3 / 37.8, 256 rows behind
+// 512 20.0 / 20.1 / 21.6.
 constexpr int64_t kTaskCost = 128;
 
 struct PlanLayout {
@@ -1137,7 +1165,10 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
             if (per) splits = div_up(keys, per);
         };
         // KV heads of one task over a row's own keys: short ones share a task, a
-        // wave or two for each, so that its cost beside the keys is paid once.
+        // wave or two for each, so that its cost beside the keys is paid once
+        // (256 rows behind 512 with up to 64 own keys: 29.6 -> 20.1 us; 64
+        // behind 2048 25.1 -> 23.7; 33 rows in 2 groups, heads of 64, 13.4 ->
+        // 13.6-14.4).
         auto heads_of = [&](int64_t keys, int64_t chunk) -> int64_t {
             if (group > kNarrow) return 1;
             for (int64_t h : {4, 2})

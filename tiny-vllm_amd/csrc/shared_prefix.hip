@@ -47,8 +47,8 @@
 // 17 %, the loads 9 %, the exponentials 3 %. Short calls are bound by chains of
 // dependent loads (plan, page, row) and by the second launch.
 // 64 queries per wave at one workgroup per CU halve the staging and were
-// slower (one wave per SIMD has nothing to run while it waits); so were narrow
-// tasks ahead of the wide ones or between them (64 rows behind 2048: 26.2 and
+// slower (one wave per SIMD has nothing to run while it waits: with 32 queries
+// 453 us instead of 340 for 256 rows behind 65536); so were narrow tasks ahead of the wide ones or between them (64 rows behind 2048: 26.2 and
 // 26.6 us; 256 behind 32768: 284 and 294).
 #include "common.h"
 

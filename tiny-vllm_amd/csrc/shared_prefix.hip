@@ -316,7 +316,7 @@ __device__ __forceinline__ void interleave() {
     static_for<0, kAhead>([&](auto m) {
         __builtin_amdgcn_sched_group_barrier(kRead, m < NC ? 1 : 2, 0);
     });
-    __builtin_amdgcn_sched_group_barrier(kValu, 20, 0);
+    __builtin_amdgcn_sched_group_barrier(kValu, 12, 0);
     static_for<0, kAll>([&](auto m) {
         __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
         if constexpr (m + kAhead < kAll)
@@ -500,8 +500,10 @@ shared_prefix_tasks(Args<T> a) {
 #pragma unroll
         for (int n = 0; n < ND; ++n) o[n] = f32x16{};
         float m_run = -INFINITY, l_run = 0.f;
-        U16x8 pb[2] = {};  // weights of the last tile, not yet multiplied with its V:
-                           // step s's token 16s + 8jj + 4*half + i at k = 4jj + i
+        // Weights of the last tile, not yet multiplied with its V (two sets: a
+        // step reads one and writes the other): step s's token 16s + 8jj +
+        // 4*half + i at k = 4jj + i.
+        U16x8 pa[2] = {}, pb[2];
         // S^T of a tile: token 8(v/4) + 4*half + v%4 of the lane's query.
         auto scores = [&](int i, f32x16& sc) {
             const uint16_t* const kt = ks + (i & 1) * K_TILE + col * K_LD + 8 * half;
@@ -512,7 +514,7 @@ shared_prefix_tasks(Args<T> a) {
         };
         const int vlane = (4 * half + ((lane & 15) >> 2)) * V_LD + 16 * ((lane >> 4) & 1) +
                           4 * (lane & 3);
-        auto values = [&](int i) {  // O^T += V^T P^T of tile i, whose weights are in pb
+        auto values = [&](int i, const U16x8 (&p)[2]) {  // O^T += V^T P^T of tile i
             const uint16_t* const vt = vs + (i & 1) * V_TILE + vlane;
 #pragma unroll
             for (int s = 0; s < 2; ++s)
@@ -521,7 +523,7 @@ shared_prefix_tasks(Args<T> a) {
                     const uint2 lo = read_transposed(vt + (16 * s) * V_LD + 32 * n);
                     const uint2 hi = read_transposed(vt + (16 * s + 8) * V_LD + 32 * n);
                     const U16x8 va = {{lo.x, lo.y, hi.x, hi.y}};
-                    o[n] = mfma_32x32x16<_Float16>(va, pb[s], o[n]);
+                    o[n] = mfma_32x32x16<_Float16>(va, p[s], o[n]);
                 }
         };
         // Step i. LDS holds K of two tiles and V of two: K of i + 1 is read while
@@ -550,7 +552,8 @@ shared_prefix_tasks(Args<T> a) {
             for (int v = 0; v < 16; ++v) mx[v & 1] = fmaxf(mx[v & 1], sc[v]);
             return pair_max(fmaxf(mx[0], mx[1])) * a.scale_log2;
         };
-        auto step = [&](Stage& st, int i, f32x16& sc, f32x16& next) {
+        auto step = [&](Stage& st, int i, f32x16& sc, f32x16& next, U16x8 (&pl)[2],
+                        U16x8 (&pn)[2]) {
             __syncthreads();
             trim(st.k, i + 2);
             trim(st.v, i);
@@ -566,8 +569,8 @@ shared_prefix_tasks(Args<T> a) {
             if (i == 0) {  // (nothing to rescale yet)
                 m_run = cm;
             } else if (__builtin_amdgcn_ballot_w64(grow)) {
-                values(i - 1);  // at the old maximum
-                pb[0] = pb[1] = U16x8{};
+                values(i - 1, pl);  // at the old maximum
+                pl[0] = pl[1] = U16x8{};
                 const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - cm) : 1.f;
                 m_run = grow ? cm : m_run;
                 l_run *= alpha;
@@ -579,7 +582,6 @@ shared_prefix_tasks(Args<T> a) {
             // not run beside the products.
             asm volatile("" : "+v"(m_run));
             scores(i + 1, next);
-            U16x8 pn[2];
             const float m_use = m_run == -INFINITY ? 0.f : m_run - kShift;
             float ps[2] = {0.f, 0.f};
 #pragma unroll
@@ -598,14 +600,12 @@ shared_prefix_tasks(Args<T> a) {
                     ps[s] = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, hw), ones, ps[s], false);
                 }
             l_run += ps[0] + ps[1];
-            values(i - 1);
+            values(i - 1, pl);
             stage(st, i);
             cm = maximum(next);
-            pb[0] = pn[0];
-            pb[1] = pn[1];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) asm volatile("" : "+v"(pb[0].w[w]), "+v"(pb[1].w[w]));
-            asm volatile("" : "+v"(cm));
+            for (int w = 0; w < 4; ++w) asm volatile("" : "+v"(pn[0].w[w]), "+v"(pn[1].w[w]));
+            asm volatile("" : "+v"(cm), "+v"(l_run));
             interleave<NC, ND>();
         };
 
@@ -667,11 +667,11 @@ shared_prefix_tasks(Args<T> a) {
         // waits to expect the first one's loads at once.
         const int steps = (ntiles + 1) & ~1;
         for (int i = 0; i < steps; i += 2) {
-            step(st0, i, sa, sb);
-            step(st1, i + 1, sb, sa);
+            step(st0, i, sa, sb, pa, pb);
+            step(st1, i + 1, sb, sa, pb, pa);
         }
         __syncthreads();  // V of the last tile
-        values(steps - 1);
+        values(steps - 1, pa);
 
         bool again = false;
         if constexpr (kConvert) {

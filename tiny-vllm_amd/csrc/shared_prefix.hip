@@ -1176,10 +1176,15 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
             return 1;
         };
         // The length of a task: the one that ends soonest by a simple estimate.
-        // Tasks run on kSlots slots, longest first: all at once where they are
+        // Tasks run on the card's slots, longest first: all at once where they are
         // that few, otherwise the slots' mean share and half of a last, short
         // task; and the parts are written and read again, an entry of 128 dims
         // in about the time of 4 keys of a slot (8 bytes a dim, 512 bytes a key).
+        // Head dims above 128 leave one workgroup to a CU. With 512 -> 256 slots,
+        // both kernels at head dim 256: 128 rows behind 16384 100 -> 91 us, 48
+        // behind 2048 (FP8) 37.2 -> 34.8, 24 behind 1024 21.3 -> 20.6, but 64
+        // behind 8192 36.9 -> 39.6.
+        const int64_t slots = head_dim > 128 ? kSlots / 2 : kSlots;
         const int64_t least = std::max(kKeyUnit, div_up(cost, kMaxSplits));
         int64_t chunk = 0;
         double best = 0;
@@ -1204,10 +1209,10 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
                     add(own_tiles * num_kv_heads / h, num_heads, own[r] * h);
                 }
             const double time =
-                (count <= kSlots ? double(longest)
-                                 : std::max(double(longest), double(sum) / kSlots +
-                                                                 0.5 * double(shortest))) +
-                double(entries) * double(head_dim) / 32 / kSlots;
+                (count <= slots ? double(longest)
+                                : std::max(double(longest), double(sum) / double(slots) +
+                                                                0.5 * double(shortest))) +
+                double(entries) * double(head_dim) / 32 / double(slots);
             if (!chunk || time < best) {
                 chunk = c;
                 best = time;

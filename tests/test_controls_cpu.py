@@ -37,6 +37,14 @@ def test_params_are_checked(wrong, error):
         SamplingParams(**wrong)
 
 
+def test_penalties_that_vanish_in_float32_are_refused():
+    """The kernel divides by the penalty in float32: 1e-46 would be 0 there."""
+    for value in (1e-46, 2.0 ** -150, 1e-39):
+        with pytest.raises(ValueError, match="positive"):
+            SamplingParams(repetition_penalty=value)
+    assert SamplingParams(repetition_penalty=2.0 ** -126).penalised
+
+
 def entry_args(**over):
     """Arguments of tvllm_logit_controls with no rows."""
     args = dict(logits=None, rows=0, vocab=100, stride=100, rep=None, pres=None, freq=None,

@@ -81,7 +81,7 @@ class SamplingParams:
             raise TypeError("ignore_eos must be bool")
         for name in ("repetition_penalty", "presence_penalty", "frequency_penalty"):
             object.__setattr__(self, name, _float32(name, getattr(self, name)))
-        if self.repetition_penalty <= 0.0:
+        if self.repetition_penalty < 2.0 ** -126:  # (float32 has it as 0, or nearly)
             raise ValueError("repetition_penalty must be positive")
         bias = self.logit_bias
         pairs = dict(bias.items() if isinstance(bias, Mapping) else bias)

@@ -217,6 +217,7 @@ int tvllm_paged_decode_noalloc(const void* q, int64_t q_token_stride,
  *   of every row of group g lie in the same blocks, the rows' tables naming
  *   them alike. lengths[r] >= prefix_lens[groups[r]]. A group of one row
  *   shares nothing. All host pointers.
+ * Few short rows are planned without sharing.
  * num_tasks receives the number of tasks (the grid; at most
  * tvllm_shared_prefix_max_tasks), workspace_bytes what the call needs (at most
  * tvllm_shared_prefix_workspace_size). A plan buffer whose contents change
@@ -244,7 +245,9 @@ int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* groups,
  * 8-element units, q rows and the plan 16-byte aligned, out rows 8-byte; out
  * is not q's memory. workspace (16-byte
  * aligned, no initialisation) holds the partial results of this call; calls
- * that may overlap need their own. fp32 softmax and sums; the weights enter
+ * that may overlap need their own. Null for a plan that needs 0 bytes and has
+ * no row without keys: the call is one launch then (any other plan writes
+ * nothing). fp32 softmax and sums; the weights enter
  * the products as two 16-bit terms of the cache's type, or, over keys shared by
  * more than 16 query vectors of a KV head, as fp16 (11 bits; 2^-32 of the
  * row's largest where that is more). An infinity or NaN in V makes the outputs

@@ -369,3 +369,105 @@ def test_refused_over_the_queries_and_under_capture(device):
     torch.cuda.synchronize()
     paged_decode_shared_prefix(q, cache, 0, meta, plan, out, scale=b["scale"])
     check(b, out)
+
+
+# Few short rows are planned without sharing; a long row beside them has the
+# groups' keys shared and their parts merged.
+LONG = (-1, 700)
+
+
+def shares(b, device):
+    """Whether the batch's plan shares a prefix (a task of more than one row)."""
+    plan = on_device(b, device)[3]
+    return plan.workspace_bytes > 0
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("count", [2, 5, 40])
+def test_one_group_beside_a_long_row(device, shape, count):
+    heads, kv_heads, dim, dtype, fp8, layout, bs = shape
+    own = [0, 1, 2, 17, 63, 64, 65, 130, 300]
+    rows = [(0, own[i % len(own)]) for i in range(count)] + [(-1, 77), (-1, 0), (-1, 1), LONG]
+    b = make_batch(seed=40 + count, heads=heads, kv_heads=kv_heads, dim=dim, dtype=dtype, fp8=fp8,
+                   layout=layout, block_size=bs, prefixes=[-(-330 // bs) * bs], rows=rows)
+    assert shares(b, device)
+    out = run(b, device)
+    assert (out[count + 1] == 0).all()
+    check(b, out)
+
+
+@pytest.mark.parametrize("dtype,fp8", [(BF16, False), (F16, False), (BF16, True)])
+def test_strided_queries_and_outputs_beside_a_long_row(device, dtype, fp8):
+    from tinyvllm.kernels.shared_prefix import paged_decode_shared_prefix
+
+    b = make_batch(seed=50, heads=8, kv_heads=2, dim=64, dtype=dtype, fp8=fp8, prefixes=[512],
+                   rows=[(0, n) for n in range(1, 30)] + [LONG])
+    q, cache, meta, plan, out = on_device(b, device)
+    packed = torch.randn(30, 12, 72, device=device).to(dtype)
+    packed[:, 2:10, :64] = q
+    spaced = torch.zeros(30, 10, 72, device=device, dtype=dtype)
+    paged_decode_shared_prefix(packed[:, 2:10, :64], cache, 0, meta, plan, spaced[:, 1:9, :64],
+                               scale=b["scale"])
+    check(b, spaced[:, 1:9, :64])
+    assert (spaced[:, 0] == 0).all() and (spaced[:, 9] == 0).all()
+    assert (spaced[..., 64:] == 0).all()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("count", [3, 40])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_unattended_slots_do_not_matter_beside_a_long_row(device, bad, count, dim):
+    rows = [(0, n) for n in (1, 3, 9, 15, 17, 31, 33, 50)] * 5
+    b = make_batch(seed=51, heads=8, kv_heads=2, dim=dim, dtype=BF16, prefixes=[208],
+                   rows=rows[:count] + [LONG])
+    assert shares(b, device)
+    want = run(b, device)
+    used = torch.zeros(len(b["k"]), dtype=torch.bool)
+    for table, n in zip(b["tables"], b["lengths"]):
+        for t in range(n):
+            used[table[t // 16] * 16 + t % 16] = True
+    for name in "kv":
+        b[name][~used] = bad
+    assert torch.equal(run(b, device), want)
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan"), 1e30])
+def test_extreme_values_of_a_shared_prefix(device, value):
+    """V beyond fp16, an infinity or a NaN in one dim of one KV head's shared
+    keys: the wide tasks that meet it are done again, others keep their values."""
+    rows = [(0, 20 + i) for i in range(24)] + [LONG]
+    b = make_batch(seed=52, heads=8, kv_heads=2, dim=128, dtype=BF16, prefixes=[400], rows=rows)
+    assert shares(b, device)
+    plain = run(b, device).cpu()
+    b["v"][b["tables"][5][130 // 16] * 16 + 130 % 16, 1, 77] = value
+    got = run(b, device).cpu()
+    hit = torch.zeros(25, 8, 128, dtype=torch.bool)
+    hit[:24, 4:, 77] = True
+    if value == 1e30:
+        check(b, got.to(device))
+    else:
+        assert not torch.isfinite(got[hit]).any()
+    clean = dict(b, v=torch.where(b["v"].abs() < 1e29, b["v"], 0))
+    want, mass, qk = attend64(clean)
+    limit = allowed(clean, want, mass, qk, BF16)
+    assert ((got.double() - want).abs()[~hit] <= limit[~hit]).all()
+    assert torch.equal(got[24], plain[24])
+
+
+def test_calls_without_parts_need_no_workspace(device):
+    """Few short rows: one launch, no workspace; with a row without keys, its
+    zeros come from the second one."""
+    rows = [(0, 5), (0, 40), (-1, 33)]
+    for more, empty in (([], False), ([(-1, 0)], True)):
+        b = make_batch(seed=53, heads=8, kv_heads=2, dim=128, dtype=BF16, prefixes=[64],
+                       rows=rows + more)
+        q, cache, meta, plan, out = on_device(b, device)
+        assert plan.workspace_bytes == 0
+        from tinyvllm.kernels.shared_prefix import paged_decode_shared_prefix
+
+        for workspace in (None, torch.empty(0, dtype=torch.uint8, device=device)):
+            out.fill_(float("nan"))
+            paged_decode_shared_prefix(q, cache, 0, meta, plan, out, scale=b["scale"],
+                                       workspace=workspace)
+            check(b, out)
+            assert not empty or (out[3] == 0).all()

@@ -82,7 +82,7 @@ constexpr float kShift = 7.f;
 // int32 words: header | per row (first part, parts) | members | tasks.
 constexpr int kHeader = 16;
 constexpr int kTaskWords = 8;
-enum Header { H_TASKS, H_ROWS, H_HEADS, H_KV_HEADS, H_DIM, H_BLOCK, H_PARTS };
+enum Header { H_TASKS, H_ROWS, H_HEADS, H_KV_HEADS, H_DIM, H_BLOCK, H_PARTS, H_MERGE };
 // A task's queries are number q_begin .. + q_count - 1 of its group's (T_QUERIES:
 // q_begin / 16 above, q_count in the lower 8 bits), query i
 // being head i % group (of the KV head) of row members[member + i / group]; its
@@ -101,6 +101,10 @@ constexpr int64_t kMaxSplits = 1024;  // tasks that splitting adds, all units to
 // 24.3 / 23.7 / 24.1 us, 49 rows in 6 groups 41.6 / 38.3 / 37.8, 256 rows behind
 // 512 20.0 / 20.1 / 21.6.
 constexpr int64_t kTaskCost = 128;
+// Contexts (at head dims up to 128) and keys of all units up to which rows are
+// not cut at all (see below).
+constexpr int64_t kDirectKeys = 640;
+constexpr int64_t kDirectTotal = 1 << 17;
 
 struct PlanLayout {
     int64_t rows_at, members_at, tasks_at, max_tasks, words;
@@ -166,7 +170,8 @@ struct PlanHead {
     __device__ bool fits(const Args<T>& a) const {
         return (w[H_ROWS] == a.num_rows) & (w[H_HEADS] == a.heads) &
                (w[H_KV_HEADS] == a.kv_heads) & (w[H_DIM] == a.head_dim) &
-               (w[H_BLOCK] == a.block_size) & (w[H_PARTS] <= a.entries);
+               (w[H_BLOCK] == a.block_size) & (w[H_PARTS] <= a.entries) &
+               (w[H_MERGE] <= (a.part_o != nullptr));
     }
 };
 __device__ __forceinline__ PlanHead load_head(const int32_t* plan) {
@@ -1151,6 +1156,24 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
         int32_t* const tasks = plan + lay.tasks_at;
         int64_t cost = 0;
         const int64_t own_tiles = div_up(group, kWide);
+        // Few short rows: each is one task a KV head that writes its output, with
+        // nothing shared, no parts and no second launch, which costs what some
+        // 500 keys of a task do (one after the other, 107 a microsecond). us a
+        // call from Python, shared -> so: 2 rows behind 512 tokens 17.5 -> 13.2,
+        // 24 behind 608 16.8 -> 14.0, 64 behind 224 17.5 -> 13.4, but 2 behind
+        // 1008 17.1 -> 17.7; head dim 256, 4 behind 288 17.4 -> 15.4, behind 512
+        // 17.6 -> 18.0. On the card alone 10.6 and a gap -> 11.4 for the first.
+        int64_t most_keys = 0, all_keys = 0, filled = 0;
+        for (int64_t r = 0; r < num_rows; ++r) {
+            most_keys = std::max(most_keys, lengths[r]);
+            all_keys += own_tiles * num_kv_heads * lengths[r];
+            filled += lengths[r] > 0;
+        }
+        const bool direct = most_keys * std::max<int64_t>(head_dim, 128) <= kDirectKeys * 128 &&
+                            all_keys <= kDirectTotal &&
+                            filled * own_tiles * num_kv_heads <= kSlots;
+        if (direct)
+            for (Group& g : gs) g.prefix = 0;
         for (int64_t r = 0; r < num_rows; ++r) {
             const int64_t g = groups[r];
             place[r] = g >= 0 ? next[g]++ : at++;
@@ -1219,6 +1242,7 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
             }
             if (c >= 4 * most) break;
         }
+        if (direct) chunk = std::max(kKeyUnit, div_up(most_keys, kKeyUnit) * kKeyUnit);
         int64_t n = 0;
         auto emit = [&](int64_t member, int64_t q0, int64_t count, int64_t kvh, int64_t heads,
                         int64_t k0, int64_t k1, int64_t part) {
@@ -1298,6 +1322,7 @@ extern "C" int tvllm_shared_prefix_plan(const int64_t* lengths, const int64_t* g
         plan[H_DIM] = int32_t(head_dim);
         plan[H_BLOCK] = int32_t(block_size);
         plan[H_PARTS] = int32_t(entries * num_heads);
+        plan[H_MERGE] = entries > 0 || filled < num_rows;  // (which fills rows without keys)
         *num_tasks = n;
         *workspace_bytes = entries * num_heads * (head_dim + 2) * 4;
         clear_error();
@@ -1401,14 +1426,15 @@ extern "C" int tvllm_paged_decode_shared_prefix(
         a.v_scale = v_scale;
         a.entries = workspace_bytes / ((head_dim + 2) * 4);
         a.part_o = static_cast<float*>(workspace);
-        a.part_ml = reinterpret_cast<float2*>(a.part_o + a.entries * head_dim);
+        if (workspace) a.part_ml = reinterpret_cast<float2*>(a.part_o + a.entries * head_dim);
         auto go = [&]<int DP>() {
             if (num_tasks) {
                 if (f8) shared_prefix_tasks<T, DP, true><<<int(num_tasks), kThreads, 0, s>>>(a);
                 else shared_prefix_tasks<T, DP, false><<<int(num_tasks), kThreads, 0, s>>>(a);
             }
-            shared_prefix_merge<T, DP>
-                <<<int(div_up(num_rows * num_heads, kThreads / 64)), kThreads, 0, s>>>(a);
+            if (workspace)
+                shared_prefix_merge<T, DP>
+                    <<<int(div_up(num_rows * num_heads, kThreads / 64)), kThreads, 0, s>>>(a);
         };
         if (head_dim <= 32) go.template operator()<32>();
         else if (head_dim <= 64) go.template operator()<64>();

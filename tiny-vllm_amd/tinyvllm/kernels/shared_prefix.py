@@ -64,6 +64,7 @@ class SharedPrefixPlan:
         self.num_rows = 0        # of the plan last made; the grid and the
         self.num_tasks = 0       # workspace that it needs
         self.workspace_bytes = 0
+        self._least = 0          # of a workspace: rows without keys need one too
 
     def update(self, context_lens: Sequence[int], row_groups: Sequence[int],
                prefix_lens: Sequence[int]) -> None:
@@ -100,6 +101,7 @@ class SharedPrefixPlan:
             self._pending = True
         self.num_rows, self.num_tasks = len(lengths), tasks.value
         self.workspace_bytes = need.value
+        self._least = need.value if need.value or lengths.all() else 16
 
 
 def find_shared_prefixes(table_ids, table_offsets, context_lens, block_size: int
@@ -187,11 +189,12 @@ def paged_decode_shared_prefix(
         if _capturing():
             tasks, need = plan.max_tasks, plan.max_workspace_bytes
         else:
-            tasks, need = plan.num_tasks, plan.workspace_bytes
-        if workspace is None or workspace.numel() < need:
+            tasks, need = plan.num_tasks, plan._least
+        if need and (workspace is None or workspace.numel() < need):
             workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        elif require_gpu(q, workspace) != device or workspace.dtype != torch.uint8 \
-                or not workspace.is_contiguous():
+        elif workspace is not None and (
+                require_gpu(q, workspace) != device or workspace.dtype != torch.uint8
+                or not workspace.is_contiguous()):
             raise RuntimeError("workspace must be contiguous uint8 on Q's device")
         # Addresses of the layer, without views of it (1.2 us each).
         skip = layer_idx % layers * strides[0] * key.element_size()

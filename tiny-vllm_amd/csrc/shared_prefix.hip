@@ -36,20 +36,21 @@
 //
 // Measured on one MI355X (kernel trace; tasks + merge, bf16 and 32 / 8 heads of
 // 128 if not said otherwise):
-//   64 rows behind 2048 shared tokens, 64-512 own           23.5 + 4.1 us
-//   256 rows behind 32768, 1-1024 own                        220 + 10.5 us
-//   16 rows behind 32768, 64 / 8 heads, FP8 cache             35 + 8.2 us
+//   64 rows behind 2048 shared tokens, 64-512 own           22.8 + 4.1 us
+//   256 rows behind 32768, 1-1024 own                        210 + 10.7 us
+//   16 rows behind 32768, 64 / 8 heads, FP8 cache             33.6 + 8.2 us
 //   own keys alone, 256 rows of 2048         6.3 TB/s (5.2 TB/s from FP8)
 // What bounds them: the wide path's step, 32 tokens by 2 x 128 queries in
-// 1.24 us on a CU, about 830 TFLOP/s over the card where a large matrix product
+// 1.2 us on a CU, about 835 TFLOP/s over the card where a large matrix product
 // reaches 1375. No unit is full (matrix 34 %, vector 42 %, LDS 27 % busy); left
 // out one at a time, staging is 21 % of it, the products with V 23 %, with K
 // 17 %, the loads 9 %, the exponentials 3 %. Short calls are bound by chains of
 // dependent loads (plan, page, row) and by the second launch.
 // 64 queries per wave at one workgroup per CU halve the staging and were
 // slower (one wave per SIMD has nothing to run while it waits: with 32 queries
-// 453 us instead of 340 for 256 rows behind 65536); so were narrow tasks ahead of the wide ones or between them (64 rows behind 2048: 26.2 and
-// 26.6 us; 256 behind 32768: 284 and 294).
+// 453 us instead of 340 for 256 rows behind 65536); so were narrow tasks ahead
+// of the wide ones or between them (64 rows behind 2048: 26.2 and 26.6 us; 256
+// behind 32768: 284 and 294).
 #include "common.h"
 
 #include <algorithm>
@@ -313,7 +314,9 @@ __device__ __forceinline__ uint32_t widen2(uint32_t w) {
 // weights' arithmetic, then one matrix instruction at a time, each followed by
 // the read of the operand four further on and a share of the vector work.
 // Without it the compiler puts each read right before the instruction that
-// waits for it.
+// waits for it (a step takes 1.29 times as long). Vector instructions ahead of
+// the first matrix one, 256 rows behind 32768: 1 218 us, 8 212, 12 210, 20 215,
+// 30 214; per matrix instruction 4 213, 5 and 6 210.
 template <int NC, int ND>
 __device__ __forceinline__ void interleave() {
     constexpr int kValu = 0x2, kMfma = 0x8, kRead = 0x100;
